@@ -1,0 +1,533 @@
+// prompt_cache.hip -- the prompt cache of include/mi_encoder.h: bookkeeping of entries and pages on the host, kernels of
+// prompt_kernels.h.
+#include "prompt_cache.h"
+
+#include <algorithm>
+#include <cstring>
+#include <memory>
+#include <mutex>
+#include <set>
+#include <vector>
+
+#include "prompt_kernels.h"
+
+using namespace mi;
+using namespace mipc;
+
+namespace {
+
+hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
+// stands for "whatever work used it is done": a page or an entry's place may be used on any stream
+void *const ANY = reinterpret_cast<void *>(~uintptr_t(0));
+
+bool capturing(void *stream) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    MI_HIP(hipStreamIsCapturing(as_stream(stream), &st));
+    return st != hipStreamCaptureStatusNone;
+}
+
+struct Entry {
+    bool live = false;
+    int len = 0;
+    std::vector<int32_t> pages;
+    void *home = nullptr;      // the stream it was made on
+    bool foreign = false;      // other streams or a captured graph read it: freeing it waits for the device
+    void *slot_tag = ANY;      // not live: the stream whose work may still read its table
+};
+
+}  // namespace
+
+struct mi_prompt_cache {
+    mi_prompt_cache_cfg cfg{};
+    int device = 0;
+    int64_t layer_stride = 0, page_stride = 0;   // elements
+    int table_ld = 0;
+    bf16_t *pages = nullptr;
+    DevBuf own, tables;
+    std::mutex mu;
+    std::vector<int32_t> ref;            // entries that hold the page
+    std::vector<void *> tag;             // of a free page: the stream whose work may still read it
+    std::set<int32_t> free_pages;
+    std::vector<Entry> entries;
+
+    Entry &at(int32_t e) {
+        MI_REQUIRE(e >= 0 && e < (int32_t)entries.size() && entries[e].live, "prompt cache: no such entry");
+        return entries[e];
+    }
+    int32_t *table(int32_t e) const { return tables.get<int32_t>() + (int64_t)e * table_ld; }
+
+    void wait_all() {                    // everything issued so far is done: whatever is free is free for every stream
+        MI_HIP(hipDeviceSynchronize());
+        for (int32_t p : free_pages) tag[p] = ANY;
+        for (Entry &e : entries)
+            if (!e.live) e.slot_tag = ANY;
+    }
+    // the n lowest free pages, fit for use on `stream` (still free: the caller takes them once its launches are out)
+    std::vector<int32_t> pick_pages(int n, void *stream) {
+        MI_REQUIRE((size_t)n <= free_pages.size(),
+                   "prompt cache: " + std::to_string(n) + " pages needed, " + std::to_string(free_pages.size()) + " free");
+        std::vector<int32_t> got(free_pages.begin(), std::next(free_pages.begin(), n));
+        for (int32_t p : got)
+            if (tag[p] != ANY && tag[p] != stream) { wait_all(); break; }
+        return got;
+    }
+    void take(int32_t p) { free_pages.erase(p); ref[p] = 1; }
+    std::vector<int32_t> pick_entries(int n, void *stream) {
+        std::vector<int32_t> got;
+        for (int32_t e = 0; e < (int32_t)entries.size() && (int)got.size() < n; ++e)
+            if (!entries[e].live) got.push_back(e);
+        MI_REQUIRE((int)got.size() == n, "prompt cache: more than max_entries (" + std::to_string(cfg.max_entries) + ") entries");
+        for (int32_t e : got)
+            if (entries[e].slot_tag != ANY && entries[e].slot_tag != stream) { wait_all(); break; }
+        return got;
+    }
+    void open(int32_t e, int len, std::vector<int32_t> pg, void *stream) {
+        Entry &x = entries[e];
+        x.live = true; x.len = len; x.pages = std::move(pg); x.home = stream; x.foreign = false; x.slot_tag = ANY;
+    }
+    void reads(Entry &e, void *stream, bool cap) {
+        if (cap || stream != e.home) e.foreign = true;
+    }
+    void copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st);
+    void set_table(int32_t e, int at_, const int32_t *val, int n, hipStream_t st);
+    void remap(const int32_t *src, const int32_t *dst, int n, hipStream_t st);
+};
+
+void mi_prompt_cache::copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st) {
+    PcCopyArgs a{};
+    a.from = from; a.to = to; a.page_stride = page_stride; a.segs = cfg.n_layers * cfg.n_kv_heads * 2; a.hd = cfg.head_dim; a.rows = rows;
+    const int64_t words = (int64_t)a.segs * rows * cfg.head_dim / 8;
+    for (int j0 = 0; j0 < n; j0 += 480) {
+        const int m = std::min(480, n - j0);
+        std::copy(src + j0, src + j0 + m, a.src);
+        std::copy(dst + j0, dst + j0 + m, a.dst);
+        hipLaunchKernelGGL(pc_copy_kernel, dim3((unsigned)((words + 1023) / 1024), (unsigned)m), dim3(256), 0, st, a);
+        MI_HIP(hipGetLastError());
+    }
+}
+
+void mi_prompt_cache::set_table(int32_t e, int at_, const int32_t *val, int n, hipStream_t st) {
+    PcTableArgs a{};
+    for (int i0 = 0; i0 < n; i0 += 960) {
+        a.n = std::min(960, n - i0);
+        a.dst = table(e) + at_ + i0;
+        std::copy(val + i0, val + i0 + a.n, a.val);
+        hipLaunchKernelGGL(pc_table_kernel, dim3(1), dim3(256), 0, st, a);
+        MI_HIP(hipGetLastError());
+    }
+}
+
+void mi_prompt_cache::remap(const int32_t *src, const int32_t *dst, int n, hipStream_t st) {
+    PcRemapArgs a{};
+    a.tables = tables.get<int32_t>();
+    a.words = (int64_t)cfg.max_entries * table_ld;
+    for (int j0 = 0; j0 < n; j0 += 480) {
+        a.n = std::min(480, n - j0);
+        std::copy(src + j0, src + j0 + a.n, a.src);
+        std::copy(dst + j0, dst + j0 + a.n, a.dst);
+        hipLaunchKernelGGL(pc_remap_kernel, dim3((unsigned)std::min<int64_t>(1024, (a.words + 255) / 256)), dim3(256), 0, st, a);
+        MI_HIP(hipGetLastError());
+    }
+}
+
+namespace {
+
+void write_args(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n, PcWriteArgs &a, void *stream) {
+    Entry &e = c->at(entry);
+    MI_REQUIRE(layer >= 0 && n_layers >= 1 && n_layers <= c->cfg.n_layers - layer, "prompt cache: layer out of range");
+    MI_REQUIRE(start >= 0 && n >= 0 && n <= e.len - start, "prompt cache: tokens out of the entry's range");
+    for (int p = start / PC_PAGE; p < (start + n + PC_PAGE - 1) / PC_PAGE; ++p)
+        MI_REQUIRE(c->ref[e.pages[p]] == 1, "prompt cache: tokens in a page that other entries share cannot be written");
+    c->reads(e, stream, capturing(stream));
+    a.pages = c->pages; a.page_stride = c->page_stride; a.layer_stride = c->layer_stride; a.table = c->table(entry);
+    a.layer = layer; a.n_layers = n_layers; a.start = start; a.n = n; a.n_kv = c->cfg.n_kv_heads; a.hd = c->cfg.head_dim;
+}
+void write_launch(const PcWriteArgs &a, void *stream) {
+    const int64_t total = (int64_t)a.n_layers * a.n * a.n_kv * (a.hd / 8) * 2, blocks = (total + 255) / 256;
+    if (!blocks) return;
+    MI_REQUIRE(blocks <= 0x7fffffff, "prompt cache: write of more than 2^31 blocks");
+    hipLaunchKernelGGL(pc_write_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), a);
+    MI_HIP(hipGetLastError());
+}
+
+// memory that a kernel on `device` may use
+bool on_device(const void *p, int device) {
+    hipPointerAttribute_t attr;
+    if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return attr.type == hipMemoryTypeManaged || (attr.type == hipMemoryTypeDevice && attr.device == device);
+}
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// checks what the kernels take for granted, and fills in their arguments
+PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const PromptForms &f) {
+    const mi_prompt_cache_cfg &g = c->cfg;
+    Entry &e = c->at(x.entry);
+    MI_REQUIRE(x.layer >= 0 && x.layer < g.n_layers, "prompt attention: layer out of range");
+    MI_REQUIRE(x.n_heads > 0 && x.n_heads % g.n_kv_heads == 0, "prompt attention: n_heads must be a multiple of the cache's n_kv_heads");
+    MI_REQUIRE(x.n_tokens >= 0 && x.n_keys >= 0 && x.n_texts >= 1, "prompt attention: negative count, or no text");
+    MI_REQUIRE(x.n_tokens <= 0x7fffff00 / x.n_heads, "prompt attention: more than 2^31 rows");
+    MI_REQUIRE(!x.n_tokens || (x.q && x.out), "null argument");
+    MI_REQUIRE(!x.n_keys || (x.k && x.v), "null argument");
+    MI_REQUIRE((x.cu_q != nullptr) == (x.cu_k != nullptr), "prompt attention: cu_q and cu_k come together");
+    MI_REQUIRE(x.cu_q || x.n_texts == 1, "prompt attention: several texts need cu_q and cu_k");
+    MI_REQUIRE(x.scale >= 0.f && x.scale < __builtin_huge_valf(), "prompt attention: scale must be finite and not negative");
+    for (const void *p : {x.q, x.k, x.v, static_cast<const void *>(x.out)}) MI_REQUIRE(aligned16(p), "prompt attention: tensors must be 16-byte aligned");
+    for (int64_t s : {x.q_token, x.q_head, x.k_token, x.k_head, x.v_token, x.v_head, x.o_token, x.o_head})
+        MI_REQUIRE(s % 8 == 0, "prompt attention: strides must be multiples of 8 elements");
+    PromptArgs a{};
+    a.q = static_cast<const bf16_t *>(x.q); a.k = static_cast<const bf16_t *>(x.k); a.v = static_cast<const bf16_t *>(x.v);
+    a.out = static_cast<bf16_t *>(x.out);
+    a.q_token = x.q_token; a.q_head = x.q_head; a.k_token = x.k_token; a.k_head = x.k_head; a.v_token = x.v_token; a.v_head = x.v_head;
+    a.o_token = x.o_token; a.o_head = x.o_head;
+    a.pages = c->pages + x.layer * c->layer_stride; a.page_stride = c->page_stride; a.table = c->table(x.entry); a.P = e.len;
+    a.n_tokens = x.n_tokens; a.n_keys = x.n_keys; a.n_texts = x.n_texts; a.cu_q = x.cu_q; a.cu_k = x.cu_k;
+    a.n_heads = x.n_heads; a.n_kv = g.n_kv_heads; a.G = x.n_heads / g.n_kv_heads; a.causal = x.causal; a.zero_rest = x.zero_rest;
+    a.scale2 = x.scale * 1.4426950408889634f;
+    a.vt = f.vt; a.inter = f.inter; a.frag = static_cast<bf16_t *>(f.frag); a.frag_mt = f.frag_mt;
+    return a;
+}
+
+template <class T, int HD>
+void attention_launch(const PromptArgs &a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.n_tokens * a.n_heads;
+    hipLaunchKernelGGL((prompt_row_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    MI_HIP(hipGetLastError());
+}
+
+}  // namespace
+
+namespace mi {
+
+int64_t prompt_attention_workspace(mi_prompt_cache *c, const mi_prompt_attn &x) {
+    std::lock_guard<std::mutex> lk(c->mu);
+    (void)attention_args(c, x, PromptForms{});
+    return 0;
+}
+
+void prompt_attention(mi_prompt_cache *c, const mi_prompt_attn &x, const PromptForms &f, void *stream) {
+    // (held over the launch: a page that this call reads is not moved or given away in between)
+    std::lock_guard<std::mutex> lk(c->mu);
+    const PromptArgs a = attention_args(c, x, f);
+    if (!x.n_tokens) return;
+    c->reads(c->at(x.entry), stream, capturing(stream));
+    const bool f16 = c->cfg.dtype == MI_DTYPE_F16, wide = c->cfg.head_dim == 128;
+    hipStream_t st = as_stream(stream);
+    if (f16) wide ? attention_launch<TF16, 128>(a, st) : attention_launch<TF16, 64>(a, st);
+    else wide ? attention_launch<TBf16, 128>(a, st) : attention_launch<TBf16, 64>(a, st);
+}
+
+void prompt_cache_write_vt(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t start, int32_t n, const void *k, int64_t k_token, bool k_inter,
+                           const void *vt, int64_t ldvt, void *stream) {
+    std::lock_guard<std::mutex> lk(c->mu);
+    PcWriteArgs a{};
+    write_args(c, entry, layer, 1, start, n, a, stream);
+    a.k = static_cast<const bf16_t *>(k); a.k_token = k_token; a.k_head = c->cfg.head_dim; a.k_inter = k_inter;
+    a.v = static_cast<const bf16_t *>(vt); a.v_token = 1; a.v_head = (int64_t)c->cfg.head_dim * ldvt; a.v_dim = ldvt;
+    write_launch(a, stream);
+}
+
+}  // namespace mi
+
+extern "C" {
+
+int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pages, mi_prompt_cache **out) {
+    return guard([&] {
+        MI_REQUIRE(cfg && out, "null argument");
+        const mi_prompt_cache_cfg &g = *cfg;
+        MI_REQUIRE(g.head_dim == 64 || g.head_dim == 128, "prompt cache: head_dim must be 64 or 128");
+        MI_REQUIRE(g.dtype == MI_DTYPE_BF16 || g.dtype == MI_DTYPE_F16, "prompt cache: dtype must be bf16 or f16");
+        MI_REQUIRE(g.n_layers > 0 && g.n_kv_heads > 0 && g.n_pages > 0 && g.max_entries > 0 && g.max_tokens >= 0, "prompt cache: bad config");
+        MI_REQUIRE(g.n_pages <= 0x7fffffff / PC_PAGE, "prompt cache: more than 2^31 tokens");
+        MI_REQUIRE((int64_t)g.n_layers * g.n_kv_heads <= 1 << 20, "prompt cache: bad config");
+        int ndev = 0;
+        if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) {
+            (void)hipGetLastError();
+            throw Error("no HIP device available: the MI355X prompt cache has no CPU fallback");
+        }
+        MI_REQUIRE(device >= 0 && device < ndev, "invalid device ordinal");
+        MI_REQUIRE(!pages || (aligned16(pages) && on_device(pages, device)), "prompt cache: pages must be 16-byte aligned memory of the device");
+        DeviceGuard dg(device);
+        auto c = std::make_unique<mi_prompt_cache>();
+        c->cfg = g;
+        c->device = device;
+        c->layer_stride = (int64_t)g.n_kv_heads * 2 * PC_PAGE * g.head_dim;
+        c->page_stride = c->layer_stride * g.n_layers;
+        c->table_ld = g.max_tokens ? (int)(((int64_t)g.max_tokens + PC_PAGE - 1) / PC_PAGE) : g.n_pages;
+        const size_t bytes = (size_t)c->page_stride * 2 * g.n_pages, tbytes = (size_t)g.max_entries * c->table_ld * 4;
+        if (!pages) {                    // zeros: what a reserved token holds before it is written is at least finite
+            pages = c->own.reserve(bytes);
+            MI_HIP(hipMemset(pages, 0, bytes));
+        }
+        c->pages = static_cast<bf16_t *>(pages);
+        MI_HIP(hipMemset(c->tables.reserve(tbytes), 0, tbytes));   // (every word of a table is a page number, whatever is read)
+        MI_HIP(hipDeviceSynchronize());
+        c->ref.assign(g.n_pages, 0);
+        c->tag.assign(g.n_pages, ANY);
+        for (int32_t p = 0; p < g.n_pages; ++p) c->free_pages.insert(c->free_pages.end(), p);
+        c->entries.resize(g.max_entries);
+        *out = c.release();
+    });
+}
+
+int mi_prompt_cache_destroy(mi_prompt_cache *c) {
+    return guard([&] {
+        if (!c) return;
+        DeviceGuard dg(c->device);
+        MI_HIP(hipDeviceSynchronize());
+        delete c;
+    });
+}
+
+int mi_prompt_cache_new(mi_prompt_cache *c, void *stream, int32_t *entry) {
+    return guard([&] {
+        MI_REQUIRE(c && entry, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot be made while the stream is captured");
+        const int32_t e = c->pick_entries(1, stream)[0];
+        c->open(e, 0, {}, stream);
+        *entry = e;
+    });
+}
+
+int mi_prompt_cache_reserve(mi_prompt_cache *c, int32_t entry, int32_t n, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot grow while the stream is captured");
+        Entry &e = c->at(entry);
+        const int64_t max_tokens = c->cfg.max_tokens ? c->cfg.max_tokens : (int64_t)c->table_ld * PC_PAGE;
+        MI_REQUIRE(n >= 0 && (int64_t)e.len + n <= max_tokens, "prompt cache: an entry holds at most " + std::to_string(max_tokens) + " tokens");
+        const int have = (int)e.pages.size(), need = (int)(((int64_t)e.len + n + PC_PAGE - 1) / PC_PAGE);
+        if (need > have) {
+            const std::vector<int32_t> got = c->pick_pages(need - have, stream);
+            if (stream != e.home) {      // (its table may be in use on the home stream)
+                c->wait_all();
+                e.foreign = true;
+            }
+            c->set_table(entry, have, got.data(), need - have, as_stream(stream));
+            for (int32_t p : got) { c->take(p); e.pages.push_back(p); }
+        }
+        e.len += n;
+    });
+}
+
+int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n, const void *k,
+                          const int64_t ks[3], const void *v, const int64_t vs[3], void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && ks && vs && (!n || (k && v)), "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(aligned16(k) && aligned16(v), "prompt cache: keys and values must be 16-byte aligned");
+        MI_REQUIRE(!n || (on_device(k, c->device) && on_device(v, c->device)), "prompt cache: memory of the cache's device only");
+        for (int i = 0; i < 3; ++i) MI_REQUIRE(ks[i] % 8 == 0 && vs[i] % 8 == 0, "prompt cache: strides must be multiples of 8 elements");
+        PcWriteArgs a{};
+        write_args(c, entry, layer, n_layers, start, n, a, stream);
+        a.k = static_cast<const bf16_t *>(k); a.k_layer = ks[0]; a.k_token = ks[1]; a.k_head = ks[2];
+        a.v = static_cast<const bf16_t *>(v); a.v_layer = vs[0]; a.v_token = vs[1]; a.v_head = vs[2]; a.v_dim = 1;
+        write_launch(a, stream);
+    });
+}
+
+int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *out, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && (out || !count), "null argument");
+        MI_REQUIRE(count >= 0, "prompt cache: negative count");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot be forked while the stream is captured");
+        Entry &e = c->at(entry);
+        if (!count) return;
+        const std::vector<int32_t> kids = c->pick_entries(count, stream);
+        const int rows = e.len % PC_PAGE, shared = e.len / PC_PAGE;
+        const std::vector<int32_t> own = rows ? c->pick_pages(count, stream) : std::vector<int32_t>();
+        hipStream_t st = as_stream(stream);
+        PcForkArgs a{};
+        a.tables = c->tables.get<int32_t>(); a.ld = c->table_ld; a.parent = entry; a.shared = shared;
+        if (!e.pages.empty())
+            for (int j0 = 0; j0 < count; j0 += 480) {
+                a.n = std::min(480, count - j0);
+                for (int j = 0; j < a.n; ++j) { a.entry[j] = kids[j0 + j]; a.own[j] = rows ? own[j0 + j] : -1; }
+                hipLaunchKernelGGL(pc_fork_kernel, dim3((unsigned)a.n), dim3(256), 0, st, a);
+                MI_HIP(hipGetLastError());
+            }
+        if (rows) {
+            const std::vector<int32_t> src(count, e.pages[shared]);
+            c->copy_pages(c->pages, c->pages, src.data(), own.data(), count, rows, st);
+        }
+        c->reads(e, stream, false);
+        const std::vector<int32_t> base(e.pages.begin(), e.pages.begin() + shared);
+        for (int j = 0; j < count; ++j) {
+            std::vector<int32_t> pg = base;
+            for (int32_t p : base) ++c->ref[p];
+            if (rows) { c->take(own[j]); pg.push_back(own[j]); }
+            c->open(kids[j], c->entries[entry].len, std::move(pg), stream);
+            out[j] = kids[j];
+        }
+    });
+}
+
+int mi_prompt_cache_copy(mi_prompt_cache *c, int32_t entry, int32_t *copy, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && copy, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot be copied while the stream is captured");
+        Entry &e = c->at(entry);
+        const int n = (int)e.pages.size();
+        const int32_t to = c->pick_entries(1, stream)[0];
+        std::vector<int32_t> own = c->pick_pages(n, stream);
+        c->set_table(to, 0, own.data(), n, as_stream(stream));
+        c->copy_pages(c->pages, c->pages, e.pages.data(), own.data(), n, PC_PAGE, as_stream(stream));
+        c->reads(e, stream, false);
+        for (int32_t p : own) c->take(p);
+        c->open(to, e.len, std::move(own), stream);
+        *copy = to;
+    });
+}
+
+int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *list, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && (list || !n) && n >= 0, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot be freed while the stream is captured");
+        bool wait = false;
+        std::set<int32_t> seen;
+        for (int32_t i = 0; i < n; ++i) {
+            const Entry &e = c->at(list[i]);
+            MI_REQUIRE(seen.insert(list[i]).second, "prompt cache: an entry is freed twice");
+            wait = wait || e.foreign || e.home != stream;
+        }
+        if (wait) c->wait_all();
+        void *const tag = wait ? ANY : stream;
+        for (int32_t i = 0; i < n; ++i) {
+            Entry &e = c->entries[list[i]];
+            for (int32_t p : e.pages)
+                if (--c->ref[p] == 0) { c->free_pages.insert(p); c->tag[p] = tag; }
+            e.live = false;
+            e.len = 0;
+            e.pages.clear();
+            e.slot_tag = tag;
+        }
+    });
+}
+
+int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
+    return guard([&] {
+        MI_REQUIRE(c, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: pages cannot be moved while the stream is captured");
+        const int32_t n = c->cfg.n_pages, used = n - (int32_t)c->free_pages.size();
+        std::vector<int32_t> dst, src;
+        for (int32_t p : c->free_pages) {
+            if (p >= used) break;
+            dst.push_back(p);
+        }
+        for (int32_t p = used; p < n && src.size() < dst.size(); ++p)
+            if (c->ref[p]) src.push_back(p);
+        if (moved) *moved = (int32_t)src.size();
+        if (src.empty()) return;
+        bool cross = false;
+        for (const Entry &e : c->entries) cross = cross || (e.live && (e.foreign || e.home != stream));
+        for (int32_t p : dst) cross = cross || (c->tag[p] != ANY && c->tag[p] != stream);
+        if (cross) c->wait_all();
+        c->copy_pages(c->pages, c->pages, src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream));
+        c->remap(src.data(), dst.data(), (int)src.size(), as_stream(stream));
+        std::vector<int32_t> to(n);
+        for (int32_t p = 0; p < n; ++p) to[p] = p;
+        for (size_t j = 0; j < src.size(); ++j) {
+            to[src[j]] = dst[j];
+            c->ref[dst[j]] = c->ref[src[j]];
+            c->ref[src[j]] = 0;
+            c->free_pages.erase(dst[j]);
+            c->free_pages.insert(src[j]);
+            c->tag[src[j]] = stream;
+        }
+        for (Entry &e : c->entries)
+            for (int32_t &p : e.pages) p = to[p];
+        if (cross) c->wait_all();        // other streams' next reads find the pages where the tables now say
+    });
+}
+
+int mi_prompt_cache_resize(mi_prompt_cache *c, void *pages, int32_t n_pages, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c, "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: the pool cannot be replaced while the stream is captured");
+        std::vector<int32_t> src, dst;
+        for (int32_t p = 0; p < c->cfg.n_pages; ++p)
+            if (c->ref[p]) { dst.push_back((int32_t)src.size()); src.push_back(p); }
+        MI_REQUIRE(n_pages > 0 && n_pages >= (int32_t)src.size(), "prompt cache: " + std::to_string(src.size()) + " pages are in use");
+        MI_REQUIRE(n_pages <= 0x7fffffff / PC_PAGE, "prompt cache: more than 2^31 tokens");
+        MI_REQUIRE(!pages || (aligned16(pages) && on_device(pages, c->device)), "prompt cache: pages must be 16-byte aligned memory of the device");
+        const size_t bytes = (size_t)c->page_stride * 2 * n_pages;
+        DevBuf own;
+        if (!pages) {
+            pages = own.reserve(bytes);
+            MI_HIP(hipMemset(pages, 0, bytes));
+        }
+        c->wait_all();
+        c->copy_pages(c->pages, static_cast<bf16_t *>(pages), src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream));
+        // (ascending, and no page goes up: a word that one launch of the list has rewritten is below all that later ones look for)
+        c->remap(src.data(), dst.data(), (int)src.size(), as_stream(stream));
+        c->wait_all();
+        std::vector<int32_t> to(c->cfg.n_pages, 0), ref(n_pages, 0);
+        for (size_t j = 0; j < src.size(); ++j) { to[src[j]] = dst[j]; ref[dst[j]] = c->ref[src[j]]; }
+        for (Entry &e : c->entries)
+            for (int32_t &p : e.pages) p = to[p];
+        c->ref = std::move(ref);
+        c->tag.assign(n_pages, ANY);
+        c->free_pages.clear();
+        for (int32_t p = (int32_t)src.size(); p < n_pages; ++p) c->free_pages.insert(c->free_pages.end(), p);
+        c->pages = static_cast<bf16_t *>(pages);
+        c->cfg.n_pages = n_pages;
+        std::swap(c->own.p, own.p);
+        std::swap(c->own.cap, own.cap);
+    });
+}
+
+int mi_prompt_cache_entry(mi_prompt_cache *c, int32_t entry, int32_t *length, int32_t *table, int32_t cap) {
+    return guard([&] {
+        MI_REQUIRE(c, "null argument");
+        std::lock_guard<std::mutex> lk(c->mu);
+        const Entry &e = c->at(entry);
+        if (length) *length = e.len;
+        if (table)
+            for (int32_t i = 0; i < cap && i < (int32_t)e.pages.size(); ++i) table[i] = e.pages[i];
+    });
+}
+
+int mi_prompt_cache_used(mi_prompt_cache *c, int32_t *used_pages, int32_t *entries) {
+    return guard([&] {
+        MI_REQUIRE(c, "null argument");
+        std::lock_guard<std::mutex> lk(c->mu);
+        if (used_pages) *used_pages = c->cfg.n_pages - (int32_t)c->free_pages.size();
+        if (entries) *entries = (int32_t)std::count_if(c->entries.begin(), c->entries.end(), [](const Entry &e) { return e.live; });
+    });
+}
+
+int mi_prompt_attention_workspace(mi_prompt_cache *c, const mi_prompt_attn *a, int64_t *bytes) {
+    return guard([&] {
+        MI_REQUIRE(c && a && bytes, "null argument");
+        *bytes = prompt_attention_workspace(c, *a);
+    });
+}
+
+int mi_prompt_attention(mi_prompt_cache *c, const mi_prompt_attn *a, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && a, "null argument");
+        DeviceGuard dg(c->device);
+        for (const void *p : {a->q, a->k, a->v, static_cast<const void *>(a->out), static_cast<const void *>(a->cu_q), static_cast<const void *>(a->cu_k)})
+            MI_REQUIRE(!p || on_device(p, c->device), "prompt attention: memory of the cache's device only");
+        prompt_attention(c, *a, PromptForms{}, stream);
+    });
+}
+
+}  // extern "C"

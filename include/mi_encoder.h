@@ -110,6 +110,91 @@ int mi_encoder_reload_env(void);
 int mi_enc_gemm_bf16(int device, int M, int N, int K, const void *A, const void *W, void *C,
                      void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Prompt cache: the keys and values of prompts, in pages, and the attention of texts that all stand behind one of them.
+ *
+ * In a causal model what a prompt's tokens compute does not depend on the text behind them, so a batch of prompted texts
+ * needs the prompt's keys and values once.  A cache is a pool of n_pages pages of MI_PROMPT_PAGE tokens:
+ *     pages [n_pages][n_layers][n_kv_heads][2: keys, values][MI_PROMPT_PAGE][head_dim]      (bf16 or f16)
+ * An ENTRY is one prompt: a length and a page table.  Entries made by mi_prompt_cache_fork share their full pages (counted);
+ * a page that is not full belongs to one entry alone, so extending an entry never changes another one.  Pages are handed out
+ * lowest number first.
+ *
+ * Streams and threads: calls are safe from several host threads.  An entry belongs to the stream it was made on; work on
+ * it from that stream is in order.  It may be read (attention, fork, copy) on other streams too, once the caller has ordered
+ * them behind its writes (as with any device buffer); pages of entries that other streams read, or that a captured graph
+ * reads, are given out again only after the device has been waited for.  mi_prompt_attention and mi_prompt_cache_write may be
+ * captured into a graph (a replay uses the entry's length as it was at the capture; the entry must live, page moves by
+ * mi_prompt_cache_compact are followed); the other calls are refused on a stream that is being captured.
+ * ------------------------------------------------------------------------------------------------------------------- */
+#define MI_PROMPT_PAGE 64
+
+typedef struct mi_prompt_cache mi_prompt_cache;
+
+typedef struct mi_prompt_cache_cfg {
+    int32_t n_layers;
+    int32_t n_kv_heads;
+    int32_t head_dim;      /* 64 or 128 */
+    int32_t dtype;         /* MI_DTYPE_BF16 or MI_DTYPE_F16 */
+    int32_t n_pages;
+    int32_t max_entries;   /* entries alive at a time */
+    int32_t max_tokens;    /* of one entry (0: all the pages hold) */
+} mi_prompt_cache_cfg;
+
+/* pages: device memory of the caller for the pool, 16-byte aligned, kept until destroy / move; NULL: the cache allocates it. */
+int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pages, mi_prompt_cache **out);
+int mi_prompt_cache_destroy(mi_prompt_cache *c);
+
+int mi_prompt_cache_new(mi_prompt_cache *c, void *stream, int32_t *entry);
+/* n more tokens at the end of an entry; their keys and values are undefined until mi_prompt_cache_write. */
+int mi_prompt_cache_reserve(mi_prompt_cache *c, int32_t entry, int32_t n, void *stream);
+/* keys and values of tokens start .. start + n - 1 of an entry, layers layer .. layer + n_layers - 1.  k and v: device, the
+ * cache's dtype, element (l, t, h, d) at l * layer_stride + t * token_stride + h * head_stride + d (strides in elements,
+ * multiples of 8; pointers 16-byte aligned).  Pages that other entries share are refused. */
+int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n,
+                          const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3], void *stream);
+/* count new entries that begin as `entry` does: full pages are shared, the used rows of the last page are copied. */
+int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *entries, void *stream);
+/* one new entry with pages of its own throughout. */
+int mi_prompt_cache_copy(mi_prompt_cache *c, int32_t entry, int32_t *copy, void *stream);
+int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *entries, void *stream);
+/* moves pages down until the used ones are 0 .. used - 1 (each page above goes to the lowest free place, lowest first). */
+int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved);
+/* compacts into another pool of n_pages pages (`pages` as for create), which replaces the old one: larger or smaller.
+ * Waits for the device. */
+int mi_prompt_cache_resize(mi_prompt_cache *c, void *pages, int32_t n_pages, void *stream);
+/* length in tokens, and the page numbers (up to `cap` of them into `table`, which may be NULL). */
+int mi_prompt_cache_entry(mi_prompt_cache *c, int32_t entry, int32_t *length, int32_t *table, int32_t cap);
+int mi_prompt_cache_used(mi_prompt_cache *c, int32_t *used_pages, int32_t *entries);
+
+/* Attention of packed texts behind the prompt `entry`: token t of a text attends to every token of the prompt and to its
+ * own text's keys,
+ *     out[t] = sum_j softmax_j(scale * q[t] . key_j) value_j,
+ * text i holding the query tokens cu_q[i] .. cu_q[i + 1] and the keys cu_k[i] .. cu_k[i + 1] (its newest; with more keys
+ * than queries the first ones are the text's past: one query per text is the single-token form).  causal: query number a of
+ * a text sees its keys 0 .. a + keys - queries; otherwise all of them.  A query that sees nothing (empty prompt, no key)
+ * gets zeros.  n_heads is a multiple of the cache's n_kv_heads: head h reads key head h / (n_heads / n_kv_heads).
+ * Masked keys and values may hold anything, infinities and NaN too. */
+typedef struct mi_prompt_attn {
+    int32_t entry, layer;
+    int32_t n_heads;
+    int32_t n_tokens, n_keys, n_texts;
+    const void *q;                   /* [n_tokens][n_heads][head_dim], the cache's dtype, device (as k, v, out) */
+    const void *k, *v;               /* [n_keys][n_kv_heads][head_dim]; may be NULL with n_keys = 0 */
+    void *out;                       /* [n_tokens][n_heads][head_dim] */
+    int64_t q_token, q_head;         /* strides in elements, multiples of 8; head_dim is contiguous */
+    int64_t k_token, k_head, v_token, v_head, o_token, o_head;
+    const int32_t *cu_q, *cu_k;      /* device, [n_texts + 1], not decreasing; both NULL: one text */
+    int32_t causal;
+    float scale;                     /* 1 / sqrt(head_dim) as a rule */
+    int32_t zero_rest;               /* tokens behind the last text: 0 left as they are, 1 zeros */
+    int32_t reserved;                /* 0 */
+    void *workspace;                 /* device, 16-byte aligned, mi_prompt_attention_workspace bytes; not shared by calls that can overlap */
+    int64_t workspace_bytes;
+} mi_prompt_attn;
+int mi_prompt_attention_workspace(mi_prompt_cache *c, const mi_prompt_attn *a, int64_t *bytes);
+int mi_prompt_attention(mi_prompt_cache *c, const mi_prompt_attn *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

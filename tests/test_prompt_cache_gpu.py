@@ -1,0 +1,488 @@
+"""GPU tests of the prompt cache (csrc/prompt_kernels.h through prompt_cache.PromptCache): the attention of packed texts behind
+a cached prompt against the formula in 64 bits, and the operations on the cache's pages against a host model of them.
+
+Tolerance of the attention, element by element, from the roundings it makes.  With w_j = p_j / sum p (the exact weights):
+  * a probability enters the product with V rounded to the tensors' type: off by at most half a step, h = finfo.eps / 2, of
+    itself, so the output by h sum w |v|;
+  * the output is rounded once: h |o|;
+  * scores, exponentials, sums and accumulators are f32.  A score of magnitude s (sum of |q k| products x scale) is off by at
+    most ~hd 2^-24 s, which moves its weight by that much: with the inputs below s < 200 and hd <= 128, 2^-24 x 128 x 200 = 1.6e-3
+    at the very worst, where every rounding goes the same way; the bound used is 4e-4 sum w |v| (a quarter of that);
+  * f16 holds 2^7 p: a probability below 2^-25 2^-7 of the largest is lost: at most 2^-32 |v| for each key (below the f32 term)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def pc():
+    import abstracts_search_amd.prompt_cache as m
+    return m
+
+
+def reference(q, pk, pv, k, v, cu_q, cu_k, causal, scale=None):
+    """(o, sum w |v|) in 64 bits; rows that see nothing are zero"""
+    hd, rep = q.shape[2], q.shape[1] // pk.shape[1]
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    o = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    b = torch.zeros_like(o)
+    for i in range(len(cu_q) - 1):
+        a0, a1, k0, k1 = cu_q[i], cu_q[i + 1], cu_k[i], cu_k[i + 1]
+        nq, nk = a1 - a0, k1 - k0
+        if not nq:
+            continue
+        kk = torch.cat([pk.double(), k[k0:k1].double()]).repeat_interleave(rep, 1)
+        vv = torch.cat([pv.double(), v[k0:k1].double()]).repeat_interleave(rep, 1)
+        P = pk.shape[0]
+        for h in range(q.shape[1]):
+            for t in range(nq):
+                n = P + (min(max(nk - nq + t + 1, 0), nk) if causal else nk)
+                if not n:
+                    continue
+                w = torch.softmax((kk[:n, h] @ q[a0 + t, h].double()) * scale, 0)
+                o[a0 + t, h] = w @ vv[:n, h]
+                b[a0 + t, h] = w @ vv[:n, h].abs()
+    return o, b
+
+
+def reference_many(q, pk, pv, k, v, cu_q, cu_k, causal, scale=None):
+    """the same by whole matrices (long cases)"""
+    hd, rep, P = q.shape[2], q.shape[1] // pk.shape[1], pk.shape[0]
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    o = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    b = torch.zeros_like(o)
+    for i in range(len(cu_q) - 1):
+        a0, a1, k0, k1 = cu_q[i], cu_q[i + 1], cu_k[i], cu_k[i + 1]
+        nq, nk = a1 - a0, k1 - k0
+        if not nq or not P + nk:
+            continue
+        kk = torch.cat([pk.double(), k[k0:k1].double()]).repeat_interleave(rep, 1)
+        vv = torch.cat([pv.double(), v[k0:k1].double()]).repeat_interleave(rep, 1)
+        s = torch.bmm(q[a0:a1].double().transpose(0, 1).contiguous(), kk.permute(1, 2, 0).contiguous()) * scale
+        if causal:
+            s[:, :, P:].masked_fill_(torch.ones(nq, nk, dtype=torch.bool, device=q.device).triu(nk - nq + 1), -math.inf)
+        w = torch.softmax(s, -1)
+        sees = P + (torch.arange(nk - nq + 1, nk + 1, device=q.device).clamp(0, nk) if causal else torch.full((nq,), nk, device=q.device))
+        w = torch.where((sees == 0).view(1, nq, 1), torch.zeros_like(w), w)
+        o[a0:a1] = torch.bmm(w, vv.transpose(0, 1).contiguous()).transpose(0, 1)
+        b[a0:a1] = torch.bmm(w, vv.abs().transpose(0, 1).contiguous()).transpose(0, 1)
+    return o, b
+
+
+def close(out, o, b, what=""):
+    h = torch.finfo(out.dtype).eps / 2
+    err = (out.double() - o).abs()
+    tol = (h + 4e-4) * b + h * o.abs() * (1 + h) + 1e-7
+    bad = ~(err <= tol)
+    assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[:5].tolist(), float(err[bad].max()), float((err / tol)[bad].max()))
+
+
+def make(pc, dtype, heads, kv, hd, prompt, lens, past=None, layers=2, layer=1, seed=0, scramble=True):
+    """a cache with a prompt in scattered pages, and packed texts"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    cache = pc.PromptCache(layers, kv, hd, -(-prompt // 64) * 2 + 6, dtype=dtype, max_entries=8)
+    pk, pv = r(layers, prompt, kv, hd), r(layers, prompt, kv, hd)
+    e = cache.new()
+    if scramble:                                              # two entries grow in turn, one of them leaves: every other page
+        other = cache.new()
+        for p0 in range(0, prompt, 64):
+            cache.extend(e, pk[:, p0:p0 + 64], pv[:, p0:p0 + 64])
+            cache.extend(other, pk[:, :1].expand(-1, 64, -1, -1), pv[:, :1].expand(-1, 64, -1, -1))
+        cache.free(other)
+    else:
+        cache.extend(e, pk, pv)
+    past = past or [0] * len(lens)
+    cu_q = np.cumsum([0] + list(lens)).tolist()
+    cu_k = np.cumsum([0] + [n + p for n, p in zip(lens, past)]).tolist()
+    q, k, v = r(cu_q[-1], heads, hd) * 1.5, r(cu_k[-1], kv, hd), r(cu_k[-1], kv, hd)
+    return cache, e, pk[layer], pv[layer], q, k, v, cu_q, cu_k
+
+
+def dev(cu):
+    return torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+
+CASES = [
+    # dtype heads kv hd prompt lens past causal
+    (BF, 12, 2, 128, 37, [10], None, True),
+    (BF, 4, 2, 64, 1, [1], None, True),
+    (HF, 8, 8, 64, 64, [1, 1, 1], [0, 5, 64], True),
+    (BF, 7, 1, 128, 65, [3, 0, 17, 1, 0], [0, 4, 2, 9, 0], True),
+    (HF, 16, 2, 128, 130, [64, 65, 63], None, True),
+    (BF, 6, 3, 64, 0, [5, 33, 1, 70], None, True),
+    (BF, 6, 3, 64, 0, [5, 33, 1, 70], [3, 0, 0, 64], False),
+    (HF, 5, 5, 128, 63, [2, 90], [61, 40], True),
+    (BF, 40, 1, 128, 128, [3, 9], [0, 1], True),              # a group of 40 heads: a token spans several tiles of rows
+    (HF, 28, 4, 128, 200, [1] * 40, list(range(40)), True),
+    (BF, 64, 8, 64, 257, [1] * 9 + [0] * 3 + [2], [0] * 12 + [7], False),
+    (BF, 2, 2, 128, 5, [129, 1, 255], [0, 300, 0], True),
+]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,hd,prompt,lens,past,causal", CASES)
+def test_attention_vs_formula(pc, dtype, heads, kv, hd, prompt, lens, past, causal):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, heads, kv, hd, prompt, lens, past)
+    out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k), causal=causal)
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, causal)
+    close(out, o, b)
+
+
+def test_the_two_references_agree(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 5, [3, 0, 6], [0, 2, 4])
+    for causal in (True, False):
+        a, b = reference(q, pk, pv, k, v, cu_q, cu_k, causal), reference_many(q, pk, pv, k, v, cu_q, cu_k, causal)
+        assert torch.allclose(a[0], b[0], rtol=1e-12, atol=1e-12) and torch.allclose(a[1], b[1], rtol=1e-12, atol=1e-12)
+
+
+def test_more_queries_than_keys_leaves_rows_empty(pc):
+    """causal, aligned at the end: with 2 keys for 5 queries the first three see no key of their own; without a prompt they are zero"""
+    for prompt in (0, 3):
+        cache, e, pk, pv, q, _, _, cu_q, _ = make(pc, BF, 4, 2, 64, prompt, [5, 4, 3])
+        cu_k = [0, 2, 2, 5]
+        k, v = torch.randn(5, 2, 64, device="cuda").to(BF), torch.randn(5, 2, 64, device="cuda").to(BF)
+        out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+        o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+        close(out, o, b)
+        if not prompt:
+            assert (out[:3] == 0).all() and (out[5:9] == 0).all() and (out[3:5] != 0).any()
+
+
+def test_no_own_keys_one_text_and_default_bounds(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, HF, 6, 2, 64, 70, [21])
+    none = torch.zeros(0, 2, 64, dtype=HF, device="cuda")
+    o, b = reference_many(q, pk, pv, none, none, [0, 21], [0, 0], True)
+    close(cache.attention(e, 1, q), o, b)
+    close(cache.attention(e, 1, q, none, none), o, b)
+    o, b = reference_many(q, pk, pv, k, v, [0, 21], [0, 21], True)
+    close(cache.attention(e, 1, q, k, v), o, b)
+    close(cache.attention(e, 1, q, k, v, dev([0, 21])), o, b)
+    o, b = reference_many(q, pk, pv, k, v, [0, 21], [0, 21], True, scale=0.3)
+    close(cache.attention(e, 1, q, k, v, scale=0.3), o, b)
+    assert cache.attention(e, 1, q[:0]).shape == (0, 6, 64)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_strided_views_of_a_fused_projection(pc, causal):
+    """q, k and v as slices of one [tokens, (heads + 2 kv) hd] buffer; out a slice too; odd strides are copied inside the call"""
+    heads, kv, hd, prompt, lens = 6, 2, 64, 77, [19, 1, 40]
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, heads, kv, hd, prompt, lens)
+    T = cu_q[-1]
+    fused = torch.cat([q, k, v], 1).contiguous()
+    big = torch.full((T, 2 * heads, hd), 7.0, dtype=BF, device="cuda")
+    fq, fk, fv = fused[:, :heads], fused[:, heads:heads + kv], fused[:, heads + kv:]
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, causal)
+    got = cache.attention(e, 1, fq, fk, fv, dev(cu_q), dev(cu_k), causal=causal, out=big[:, heads:])
+    close(got, o, b)
+    assert (big[:, :heads] == 7).all()
+    odd = torch.zeros(T, heads, hd + 1, dtype=BF, device="cuda")[:, :, 1:]      # rows of 65 elements, 2 bytes off
+    odd.copy_(q)
+    turned = k.permute(1, 0, 2).contiguous().permute(1, 0, 2)                   # heads outermost
+    last = v.permute(0, 2, 1).contiguous().permute(0, 2, 1)                     # the last axis strided
+    assert torch.equal(cache.attention(e, 1, odd, turned, last, dev(cu_q), dev(cu_k), causal=causal), got)
+
+
+def test_rows_behind_the_last_text(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 6, 2, 128, 90, [30, 5])
+    pad = torch.randn(9, 6, 128, device="cuda").to(BF)
+    padk = torch.full((9, 2, 128), float("nan"), dtype=BF, device="cuda")
+    q2, k2, v2 = torch.cat([q, pad]), torch.cat([k, padk]), torch.cat([v, padk])
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    out = cache.attention(e, 1, q2, k2, v2, dev(cu_q), dev(cu_k))
+    close(out[:35], o, b)
+    assert (out[35:] == 0).all()
+    held = torch.full_like(q2, 3.0)
+    cache.attention(e, 1, q2, k2, v2, dev(cu_q), dev(cu_k), out=held)
+    assert torch.equal(held[:35], out[:35]) and (held[35:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,kv,hd,prompt,lens", [(12, 2, 128, 70, [9, 30, 64, 1, 50]), (4, 4, 64, 0, [3, 1, 1, 20])])
+def test_what_is_masked_may_hold_anything(pc, dtype, heads, kv, hd, prompt, lens):
+    """infinities and NaN in the keys and values of later tokens and of other texts leave every row as it was; the rows that
+    do see them get what the formula gives"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, heads, kv, hd, prompt, lens)
+    clean = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+    k2, v2 = k.clone(), v.clone()
+    for i, x in ((1, float("nan")), (3, float("inf")), (len(lens) - 1, float("-inf"))):
+        at = cu_k[i + 1] - 1                                    # a text's last key: seen by its last query alone
+        v2[at] = x
+        k2[at] = -x
+    out = cache.attention(e, 1, q, k2, v2, dev(cu_q), dev(cu_k))
+    hit = torch.zeros(cu_q[-1], dtype=torch.bool, device="cuda")
+    for i in (1, 3, len(lens) - 1):
+        hit[cu_q[i + 1] - 1] = True
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    close(out[~hit], o[~hit], b[~hit])
+    close(clean, o, b)
+    assert torch.isnan(out[cu_q[2] - 1]).all()                  # (NaN keys and values)
+    # a key of the type's lowest value, and one that is -inf in every product, weigh nothing
+    low = torch.finfo(dtype).min
+    k3, q3 = k.clone(), q.abs() + 0.01
+    k3[cu_k[1] - 1], k3[cu_k[2] - 1] = low, float("-inf")
+    out = cache.attention(e, 1, q3, k3, v, dev(cu_q), dev(cu_k))
+    o, b = reference_many(q3, pk, pv, k3, v, cu_q, cu_k, True)
+    ok = ~torch.isnan(o).any(-1).any(-1)                        # (a text whose only key is -inf has no softmax: NaN on both sides)
+    close(out[ok], o[ok], b[ok])
+    assert torch.isnan(out[~ok]).all()
+
+
+def test_extreme_scores(pc):
+    """scores far apart (a one-hot softmax), all equal, and a maximum that grows all along the prompt"""
+    for dtype in (BF, HF):
+        cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, 4, 2, 64, 300, [10, 70], scramble=False)
+        for scale in (0.0, 4.0):
+            o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True, scale=scale)
+            out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k), scale=scale)
+            # (scale 4: scores up to ~200: 32 x the f32 term of the ordinary scale, see the tolerance above)
+            h = torch.finfo(dtype).eps / 2
+            assert ((out.double() - o).abs() <= (h + 1.6e-3) * b + h * o.abs() * (1 + h) + 1e-7).all()
+        ramp = torch.linspace(0.01, 3, 300, device="cuda")[:, None, None].expand(300, 2, 64).to(dtype)
+        grow = cache.new()
+        cache.extend(grow, ramp.expand(2, 300, 2, 64), pv.expand(2, 300, 2, 64))
+        qq = torch.ones_like(q)
+        o, b = reference_many(qq, ramp, pv, k, v, cu_q, cu_k, True)
+        close(cache.attention(grow, 1, qq, k, v, dev(cu_q), dev(cu_k)), o, b)
+
+
+def test_long_prompt_few_rows_and_many(pc):
+    """single tokens over a long prompt (the work is split along it), and enough rows to fill the chip"""
+    for dtype, heads, kv, hd, prompt, lens, past in ((BF, 32, 8, 128, 20001, [1, 1, 1], [0, 31, 2]), (HF, 12, 2, 128, 9000, [7], None),
+                                                     (BF, 16, 16, 64, 1000, [200, 1, 333, 64], None), (HF, 12, 2, 128, 400, [500, 77, 300, 90, 512], None)):
+        cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, heads, kv, hd, prompt, lens, past, scramble=False)
+        for causal in (True, False):
+            o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, causal)
+            out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k), causal=causal)
+            close(out, o, b, (heads, prompt, causal))
+            assert torch.equal(out, cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k), causal=causal))   # the same bits every time
+
+
+def test_more_texts_than_a_table_in_shared_memory(pc):
+    lens = [(i * 7) % 3 for i in range(3000)]
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 20, lens)
+    out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+    g = torch.Generator().manual_seed(1)
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    close(out, o, b)
+
+
+def test_bounds_that_are_no_bounds_stay_inside(pc):
+    """cu arrays are device data nobody checks: wrong ones give wrong rows, not reads outside (texts past the end are cut)"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [30, 20])
+    for cq, ck in (([0, 30, 90], [0, 30, 90]), ([0, 30, 50], [0, 1 << 30, 1 << 30]), ([0, 30, 50], [-5, 30, -7]), ([5, 3, 50], [0, 30, 50])):
+        out = cache.attention(e, 1, q, k, v, dev(cq), dev(ck))
+        assert out.shape == q.shape
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------------------------------------------
+class Model:
+    """what the entries hold, on the host"""
+
+    def __init__(self):
+        self.kv = {}
+
+    def check(self, pc, cache):
+        held = {}
+        for e, (k, v) in self.kv.items():
+            assert cache.length(e) == k.shape[1]
+            t = cache.table(e)
+            assert len(t) == -(-k.shape[1] // 64) and all(0 <= p < cache.n_pages for p in t)
+            for i, p in enumerate(t):
+                rows = min(64, k.shape[1] - 64 * i)
+                page = cache.pages[p]
+                assert torch.equal(page[:, :, 0, :rows].transpose(1, 2).cpu(), k[:, 64 * i:64 * i + rows]), (e, i)
+                assert torch.equal(page[:, :, 1, :rows].transpose(1, 2).cpu(), v[:, 64 * i:64 * i + rows]), (e, i)
+                held.setdefault(p, []).append((e, rows))
+        for p, who in held.items():                             # only full pages are shared
+            assert len(who) == 1 or all(r == 64 for _, r in who)
+        assert cache.used_pages == len(held)
+
+
+@pytest.mark.parametrize("dtype,layers,kv,hd", [(BF, 3, 2, 64), (HF, 1, 5, 128)])
+def test_pages_against_a_model(pc, dtype, layers, kv, hd):
+    """two hundred operations in a fixed random order; after each, every entry holds what it should"""
+    rng = np.random.default_rng(3)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache, m = pc.PromptCache(layers, kv, hd, 40, dtype=dtype, max_entries=12), Model()
+    full = 0
+    for step in range(200):
+        op = rng.choice(["new", "extend", "extend", "fork", "copy", "free", "compact", "resize", "write"])
+        live = sorted(m.kv)
+        e = int(rng.choice(live)) if live else None
+        try:
+            if op == "new" or e is None:
+                n = cache.new()
+                assert n not in m.kv
+                m.kv[n] = (torch.zeros(layers, 0, kv, hd, dtype=dtype),) * 2
+            elif op == "extend":
+                n = int(rng.choice([0, 1, 5, 63, 64, 65, 200]))
+                k, v = (torch.randn(layers, n, kv, hd, generator=g, device="cuda").to(dtype) for _ in range(2))
+                cache.extend(e, k, v)
+                m.kv[e] = tuple(torch.cat([a, b.cpu()], 1) for a, b in zip(m.kv[e], (k, v)))
+            elif op == "fork":
+                kids = cache.fork(e, int(rng.integers(0, 4)))
+                assert not set(kids) & set(m.kv) and len(set(kids)) == len(kids)
+                for c in kids:
+                    m.kv[c] = m.kv[e]
+            elif op == "copy":
+                c = cache.copy(e)
+                m.kv[c] = m.kv[e]
+                assert not set(cache.table(c)) & set(cache.table(e))
+            elif op == "free":
+                cache.free(e)
+                del m.kv[e]
+            elif op == "compact":
+                cache.compact()
+                assert all(p < cache.used_pages for x in m.kv for p in cache.table(x))
+            elif op == "resize":
+                cache.resize(max(1, cache.used_pages, int(rng.integers(20, 50))))
+                assert all(p < cache.used_pages for x in m.kv for p in cache.table(x))
+            elif op == "write":
+                n = m.kv[e][0].shape[1]
+                if n % 64:                                      # the last, partly filled page is the entry's own
+                    s = n - n % 64
+                    k, v = (torch.randn(1, n - s, kv, hd, generator=g, device="cuda").to(dtype) for _ in range(2))
+                    cache.write(e, k, v, s, layer=layers - 1)
+                    kk, vv = m.kv[e][0].clone(), m.kv[e][1].clone()
+                    kk[layers - 1, s:], vv[layers - 1, s:] = k[0].cpu(), v[0].cpu()
+                    m.kv[e] = (kk, vv)
+        except RuntimeError as err:                             # a full pool or list of entries refuses and changes nothing
+            assert "free" in str(err) or "max_entries" in str(err), err
+            full += 1
+            cache.free([x for x in live[::2]])
+            for x in live[::2]:
+                del m.kv[x]
+        m.check(pc, cache)
+    assert full >= 2
+
+
+def test_pages_are_handed_out_lowest_first_and_shared(pc):
+    cache = pc.PromptCache(1, 2, 64, 12)
+    t = torch.randn(1, 130, 2, 64, device="cuda").to(BF)
+    a = cache.new()
+    cache.extend(a, t, t)
+    kids = cache.fork(a, 3)
+    assert cache.table(a) == [0, 1, 2] and [cache.table(x) for x in kids] == [[0, 1, 3], [0, 1, 4], [0, 1, 5]]
+    cache.free([a, kids[1]])
+    assert cache.used_pages == 4
+    b = cache.new()
+    cache.extend(b, t[:, :100], t[:, :100])
+    assert cache.table(b) == [2, 4]
+    cache.free(kids[0])
+    assert cache.compact() == 1 and sorted(sum((cache.table(x) for x in (kids[2], b)), [])) == [0, 1, 2, 3, 4]
+    assert cache.compact() == 0
+    with pytest.raises(RuntimeError, match="free"):
+        cache.reserve(b, 64 * 10)
+    assert cache.length(b) == 100
+
+
+def test_strided_keys_and_values_are_stored(pc):
+    cache = pc.PromptCache(2, 2, 64, 8)
+    e = cache.new()
+    x = torch.randn(2, 70, 3, 2, 64, device="cuda").to(BF)
+    cache.extend(e, x[:, :, 1], x[:, :, 2])                     # slices of a fused buffer
+    p = cache.pages[cache.table(e)].transpose(0, 1).transpose(1, 2)
+    assert torch.equal(cache.pages[0][:, :, 0].transpose(1, 2), x[:, :64, 1]) and torch.equal(cache.pages[1][:, :, 1, :6].transpose(1, 2), x[:, 64:, 2])
+    odd = torch.randn(2, 5, 2, 65, device="cuda").to(BF)[..., 1:]
+    cache.extend(e, odd, odd)
+    assert torch.equal(cache.pages[1][:, :, 0, 6:11].transpose(1, 2), odd)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# streams, graphs, refusals
+# ---------------------------------------------------------------------------------------------------------------
+def test_a_captured_pass_follows_its_inputs_and_moved_pages(pc):
+    """two graphs over one cache, replayed in turn with eager work between; a page move in between is followed"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 12, 2, 128, 5000, [1, 1, 9])
+    _, _, _, _, q2, k2, v2, cu_q2, cu_k2 = make(pc, BF, 12, 2, 128, 70, [40, 3], seed=5)
+    args = [(q, k, v, dev(cu_q), dev(cu_k)), (q2, k2, v2, dev(cu_q2), dev(cu_k2))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a in args:
+            cache.attention(e, 1, *a)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for a in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(cache.attention(e, 1, *a))
+        graphs.append(g)
+    for rep in range(4):
+        for a, g, o in zip(args, graphs, outs):
+            a[0].mul_(-0.9)
+            g.replay()
+            want = cache.attention(e, 1, *a)
+            torch.cuda.synchronize()
+            assert torch.equal(o, want), rep
+        if rep == 1:
+            assert cache.compact() > 0
+    with pytest.raises(RuntimeError, match="captured"):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            cache.fork(e)
+    torch.cuda.synchronize()
+
+
+def test_another_stream_and_freed_pages(pc):
+    """an entry read on a side stream is freed and its pages refilled at once: the reader still sees what was there"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 32, 8, 128, 8000, [40, 60], scramble=False)
+    want = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    cq, ck = dev(cu_q), dev(cu_k)
+    with torch.cuda.stream(side):
+        outs = [cache.attention(e, 1, q, k, v, cq, ck) for _ in range(8)]
+    cache.free(e)
+    f = cache.new()
+    z = torch.zeros(2, 8000, 8, 128, dtype=BF, device="cuda")
+    cache.extend(f, z, z)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_refusals(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [5])
+    bad = [
+        (ValueError, dict(q=q[0])), (ValueError, dict(q=q.half())), (ValueError, dict(q=q.cpu())), (ValueError, dict(q=q[..., :32])),
+        (RuntimeError, dict(q=torch.zeros(5, 3, 64, dtype=BF, device="cuda"))), (ValueError, dict(k=k[:4])), (ValueError, dict(v=None)),
+        (ValueError, dict(k=k[:, :1])), (ValueError, dict(cu_q=dev(cu_q).long())), (ValueError, dict(cu_q=dev([0]), cu_k=dev([0]))),
+        (ValueError, dict(cu_q=None)), (ValueError, dict(cu_k=torch.tensor(cu_k, dtype=torch.int32))), (ValueError, dict(out=q.float())),
+        (ValueError, dict(out=torch.empty(5, 4, 65, dtype=BF, device="cuda")[..., :64])), (ValueError, dict(scale=float("nan"))),
+        (ValueError, dict(scale=-1.0)), (RuntimeError, dict(entry=e + 1)), (RuntimeError, dict(entry=-1)), (RuntimeError, dict(layer=2)),
+        (RuntimeError, dict(layer=-1)), (ValueError, dict(q=q.clone().requires_grad_())),
+    ]
+    for kind, change in bad:
+        a = dict(entry=e, layer=1, q=q, k=k, v=v, cu_q=dev(cu_q), cu_k=dev(cu_k))
+        a.update(change)
+        with pytest.raises(kind):
+            cache.attention(**a)
+    with torch.no_grad():
+        assert cache.attention(e, 1, q.clone().requires_grad_(), k, v, dev(cu_q)).shape == q.shape
+    t = torch.zeros(2, 3, 2, 64, dtype=BF, device="cuda")
+    for kind, f in ((RuntimeError, lambda: cache.write(e, t, t, 68)), (RuntimeError, lambda: cache.write(e, t, t, -1)), (RuntimeError, lambda: cache.write(e, t, t, 0, layer=1)),
+                    (ValueError, lambda: cache.extend(e, t[:1], t[:1])), (ValueError, lambda: cache.extend(e, t, t[:, :2])), (ValueError, lambda: cache.extend(e, t.half(), t.half())),
+                    (RuntimeError, lambda: cache.free([e, e])), (RuntimeError, lambda: cache.free(99)), (ValueError, lambda: cache.fork(e, -1)),
+                    (RuntimeError, lambda: cache.fork(e, 99)), (RuntimeError, lambda: cache.reserve(e, -1)), (RuntimeError, lambda: cache.resize(1)),
+                    (ValueError, lambda: cache.resize(0)), (RuntimeError, lambda: cache.length(77))):
+        with pytest.raises(kind):
+            f()
+    kid = cache.fork(e)[0]
+    with pytest.raises(RuntimeError, match="share"):
+        cache.write(kid, t, t, 0)
+    cache.write(kid, t, t, 66)
+    small = pc.PromptCache(1, 2, 64, 4, max_tokens=100)
+    x = small.new()
+    with pytest.raises(RuntimeError, match="at most 100"):
+        small.reserve(x, 101)
+    small.reserve(x, 100)
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)    # nothing of this has changed the prompt
+    close(cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k)), o, b)
