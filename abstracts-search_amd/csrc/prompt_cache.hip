@@ -185,16 +185,44 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     a.pages = c->pages + x.layer * c->layer_stride; a.page_stride = c->page_stride; a.table = c->table(x.entry); a.P = e.len;
     a.n_tokens = x.n_tokens; a.n_keys = x.n_keys; a.n_texts = x.n_texts; a.cu_q = x.cu_q; a.cu_k = x.cu_k;
     a.n_heads = x.n_heads; a.n_kv = g.n_kv_heads; a.G = x.n_heads / g.n_kv_heads; a.causal = x.causal; a.zero_rest = x.zero_rest;
-    a.scale2 = x.scale * 1.4426950408889634f;
+    a.scale2 = std::max(x.scale * 1.4426950408889634f, 1e-30f);   // (0 means equal weights; a masked score is -inf, and 0 x inf is no number)
     a.vt = f.vt; a.inter = f.inter; a.frag = static_cast<bf16_t *>(f.frag); a.frag_mt = f.frag_mt;
     return a;
 }
 
-template <class T, int HD>
-void attention_launch(const PromptArgs &a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.n_tokens * a.n_heads;
-    hipLaunchKernelGGL((prompt_row_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+// how a call is cut up: waves of a workgroup (32 rows each) and splits of the keys
+struct Plan {
+    int nw, splits, tiles;
+    int64_t rows;                        // of all key heads
+    int64_t o_bytes, bytes;              // partials, workspace
+};
+Plan plan_of(const PromptArgs &a, int hd) {
+    Plan p{};
+    const int64_t per_head = (int64_t)a.n_tokens * a.G;
+    p.rows = per_head * a.n_kv;
+    p.nw = per_head <= 32 ? 1 : per_head <= 64 ? 2 : per_head <= 1024 ? 4 : 8;
+    p.tiles = (int)((per_head + 32 * p.nw - 1) / (32 * p.nw));
+    const int64_t wgs = (int64_t)p.tiles * a.n_kv, chunks = (a.P + PC_PAGE - 1) / PC_PAGE + (a.n_keys / a.n_texts + PC_PAGE - 1) / PC_PAGE;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / wgs, chunks / 2));
+    p.o_bytes = p.splits > 1 ? p.splits * p.rows * hd * 4 : 0;
+    p.bytes = p.splits > 1 ? p.o_bytes + p.splits * p.rows * 8 : 0;
+    return p;
+}
+
+template <class T, int HD, bool VT>
+void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
+    const dim3 grid((unsigned)(((int64_t)p.tiles * p.splits * a.n_kv + 7) / 8 * 8));
+    switch (p.nw) {
+        case 1: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT>), grid, dim3(64), 0, st, a); break;
+        case 2: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT>), grid, dim3(128), 0, st, a); break;
+        case 4: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT>), grid, dim3(256), 0, st, a); break;
+        default: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 8, VT>), grid, dim3(512), 0, st, a); break;
+    }
     MI_HIP(hipGetLastError());
+    if (p.splits > 1) {
+        hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)((p.rows * (HD / 4) + 255) / 256)), dim3(256), 0, st, a);
+        MI_HIP(hipGetLastError());
+    }
 }
 
 }  // namespace
@@ -203,20 +231,28 @@ namespace mi {
 
 int64_t prompt_attention_workspace(mi_prompt_cache *c, const mi_prompt_attn &x) {
     std::lock_guard<std::mutex> lk(c->mu);
-    (void)attention_args(c, x, PromptForms{});
-    return 0;
+    const PromptArgs a = attention_args(c, x, PromptForms{});
+    return x.n_tokens ? plan_of(a, c->cfg.head_dim).bytes : 0;
 }
 
 void prompt_attention(mi_prompt_cache *c, const mi_prompt_attn &x, const PromptForms &f, void *stream) {
     // (held over the launch: a page that this call reads is not moved or given away in between)
     std::lock_guard<std::mutex> lk(c->mu);
-    const PromptArgs a = attention_args(c, x, f);
+    PromptArgs a = attention_args(c, x, f);
     if (!x.n_tokens) return;
-    c->reads(c->at(x.entry), stream, capturing(stream));
     const bool f16 = c->cfg.dtype == MI_DTYPE_F16, wide = c->cfg.head_dim == 128;
+    const Plan p = plan_of(a, c->cfg.head_dim);
+    MI_REQUIRE(!p.bytes || (x.workspace && aligned16(x.workspace) && x.workspace_bytes >= p.bytes),
+               "prompt attention: a workspace of " + std::to_string(p.bytes) + " bytes is needed (mi_prompt_attention_workspace)");
+    MI_REQUIRE(!f.vt || !f16, "prompt attention: V^T operands are bf16");
+    a.splits = p.splits; a.tiles = p.tiles;
+    a.part_o = static_cast<float *>(x.workspace);
+    a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(x.workspace) + p.o_bytes);
+    c->reads(c->at(x.entry), stream, capturing(stream));
     hipStream_t st = as_stream(stream);
-    if (f16) wide ? attention_launch<TF16, 128>(a, st) : attention_launch<TF16, 64>(a, st);
-    else wide ? attention_launch<TBf16, 128>(a, st) : attention_launch<TBf16, 64>(a, st);
+    if (f16) wide ? attention_launch<TF16, 128, false>(a, p, st) : attention_launch<TF16, 64, false>(a, p, st);
+    else if (f.vt) wide ? attention_launch<TBf16, 128, true>(a, p, st) : attention_launch<TBf16, 64, true>(a, p, st);
+    else wide ? attention_launch<TBf16, 128, false>(a, p, st) : attention_launch<TBf16, 64, false>(a, p, st);
 }
 
 void prompt_cache_write_vt(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t start, int32_t n, const void *k, int64_t k_token, bool k_inter,
@@ -524,7 +560,8 @@ int mi_prompt_attention(mi_prompt_cache *c, const mi_prompt_attn *a, void *strea
     return guard([&] {
         MI_REQUIRE(c && a, "null argument");
         DeviceGuard dg(c->device);
-        for (const void *p : {a->q, a->k, a->v, static_cast<const void *>(a->out), static_cast<const void *>(a->cu_q), static_cast<const void *>(a->cu_k)})
+        for (const void *p : {a->q, a->k, a->v, static_cast<const void *>(a->out), static_cast<const void *>(a->cu_q), static_cast<const void *>(a->cu_k),
+                              static_cast<const void *>(a->workspace)})
             MI_REQUIRE(!p || on_device(p, c->device), "prompt attention: memory of the cache's device only");
         prompt_attention(c, *a, PromptForms{}, stream);
     });
