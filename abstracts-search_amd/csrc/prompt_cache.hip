@@ -177,6 +177,8 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     for (const void *p : {x.q, x.k, x.v, static_cast<const void *>(x.out)}) MI_REQUIRE(aligned16(p), "prompt attention: tensors must be 16-byte aligned");
     for (int64_t s : {x.q_token, x.q_head, x.k_token, x.k_head, x.v_token, x.v_head, x.o_token, x.o_head})
         MI_REQUIRE(s % 8 == 0, "prompt attention: strides must be multiples of 8 elements");
+    MI_REQUIRE(std::max(std::abs(x.k_token), std::abs(x.v_token)) < 1 << 23 && x.k_token >= 0 && x.v_token >= 0,
+               "prompt attention: tokens of k and v must be less than 2^23 elements apart");
     PromptArgs a{};
     a.q = static_cast<const bf16_t *>(x.q); a.k = static_cast<const bf16_t *>(x.k); a.v = static_cast<const bf16_t *>(x.v);
     a.out = static_cast<bf16_t *>(x.out);
@@ -190,7 +192,9 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     return a;
 }
 
-// how a call is cut up: waves of a workgroup (32 rows each) and splits of the keys
+// How a call is cut up.  Rows of a workgroup: 32, 64 or 128 (a wave each 32), as few as hold a key head's rows.  Where the tiles do
+// not fill the chip, the keys are split so that they nearly do (two workgroups a CU) --
+// at least two chunks of 64 keys each, or the join costs more than it saves.
 struct Plan {
     int nw, splits, tiles;
     int64_t rows;                        // of all key heads
@@ -200,7 +204,7 @@ Plan plan_of(const PromptArgs &a, int hd) {
     Plan p{};
     const int64_t per_head = (int64_t)a.n_tokens * a.G;
     p.rows = per_head * a.n_kv;
-    p.nw = per_head <= 32 ? 1 : per_head <= 64 ? 2 : per_head <= 1024 ? 4 : 8;
+    p.nw = per_head <= 32 ? 1 : per_head <= 64 ? 2 : 4;
     p.tiles = (int)((per_head + 32 * p.nw - 1) / (32 * p.nw));
     const int64_t wgs = (int64_t)p.tiles * a.n_kv, chunks = (a.P + PC_PAGE - 1) / PC_PAGE + (a.n_keys / a.n_texts + PC_PAGE - 1) / PC_PAGE;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / wgs, chunks / 2));
@@ -212,15 +216,14 @@ Plan plan_of(const PromptArgs &a, int hd) {
 template <class T, int HD, bool VT>
 void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)p.tiles * p.splits * a.n_kv + 7) / 8 * 8));
-    switch (p.nw) {
-        case 1: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT>), grid, dim3(64), 0, st, a); break;
-        case 2: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT>), grid, dim3(128), 0, st, a); break;
-        case 4: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT>), grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 8, VT>), grid, dim3(512), 0, st, a); break;
-    }
+    if (p.nw == 1) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT>), grid, dim3(64), 0, st, a);
+    else if (p.nw == 2) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT>), grid, dim3(128), 0, st, a);
+    else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT>), grid, dim3(256), 0, st, a);
     MI_HIP(hipGetLastError());
     if (p.splits > 1) {
-        hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)((p.rows * (HD / 4) + 255) / 256)), dim3(256), 0, st, a);
+        constexpr int per_wg = 256 / (HD / 4);                                    // groups of lanes
+        if (p.splits > 8) hipLaunchKernelGGL((prompt_join_kernel<T, HD, 8>), dim3((unsigned)((p.rows + per_wg / 8 - 1) / (per_wg / 8))), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((prompt_join_kernel<T, HD, 1>), dim3((unsigned)((p.rows + per_wg - 1) / per_wg)), dim3(256), 0, st, a);
         MI_HIP(hipGetLastError());
     }
 }
@@ -246,6 +249,7 @@ void prompt_attention(mi_prompt_cache *c, const mi_prompt_attn &x, const PromptF
                "prompt attention: a workspace of " + std::to_string(p.bytes) + " bytes is needed (mi_prompt_attention_workspace)");
     MI_REQUIRE(!f.vt || !f16, "prompt attention: V^T operands are bf16");
     a.splits = p.splits; a.tiles = p.tiles;
+    a.r_tiles = 1.0f / (float)p.tiles; a.r_splits = 1.0f / (float)p.splits; a.r_G = 1.0f / (float)a.G;
     a.part_o = static_cast<float *>(x.workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(x.workspace) + p.o_bytes);
     c->reads(c->at(x.entry), stream, capturing(stream));

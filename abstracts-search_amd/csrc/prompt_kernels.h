@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 namespace mipc {
 
@@ -39,6 +41,12 @@ typedef __attribute__((ext_vector_type(4))) short i16x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// f(0), f(1), .. with the numbers as types: unrolled whatever the body's size
+template <class F, int... I>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F &&f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F &&f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 
 struct TBf16 {
     static __device__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -87,9 +95,20 @@ struct PromptArgs {
     int frag_mt;
     // the tile kernel: keys split `splits` ways; partials o [splits][n_heads n_tokens][hd] and (m, sum) in f32 (splits > 1)
     int splits, tiles;
+    float r_tiles, r_splits, r_G;        // 1 / tiles, ..
     float *part_o;
     float2 *part_ml;
 };
+
+// n / d for 0 <= n < 2^31, r = 1 / d: two approximations and a correction, a dozen instructions where a division is forty
+__device__ __forceinline__ int quotient(int n, int d, float r) {
+    int q = (int)((float)n * r);
+    int rem = n - q * d;                                      // |rem| < 2^9 d
+    const int more = (int)((float)rem * r);
+    q += more;
+    rem -= more * d;
+    return q + (rem >= d) - (rem < 0);
+}
 
 // the text of token t, and the keys [lo, hi) of its own that it sees; t behind the last text: false.  Whatever the two arrays
 // hold, the result stays inside [0, n_keys].
@@ -195,16 +214,23 @@ __device__ void prompt_row(const PromptArgs &a, int token, int head, int64_t p0,
 // A masked key has p = 0 exactly, and 0 x (inf or NaN in its V) would be NaN: a row whose result is no finite number is done again
 // by prompt_row, which reads only what the row sees.
 // ---------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void dma16(const void *gptr, void *lds_wave_base) {   // 64 lanes x 16 bytes -> 1 KiB at lds_wave_base
-    const unsigned m0v = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void *)lds_wave_base);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n" ::"s"(m0v), "v"(gptr) : "memory");
+typedef __attribute__((address_space(3))) bf16_t lds_t;
+// 64 lanes x 16 bytes from base + the lane's offset -> 1 KiB at dst (the same in every lane)
+__device__ __forceinline__ void dma16(const void *base, unsigned offset, lds_t *dst) {
+    const unsigned m0v = __builtin_amdgcn_readfirstlane((unsigned)(size_t)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n" ::"s"(m0v), "v"(offset), "s"(base) : "memory");
 }
-__device__ __forceinline__ u32x2 lds_tr(const bf16_t *p) {
+// a pointer that is the same in every lane, in scalar registers
+__device__ __forceinline__ const bf16_t *uniform(const bf16_t *p) {
+    const uint64_t u = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const bf16_t *>((uint64_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)u));
+}
+__device__ __forceinline__ u32x2 lds_tr(const lds_t *p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)p));
 }
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ u32x4 lds_16(const lds_t *p) { return *(const __attribute__((address_space(3))) u32x4 *)p; }
 
-constexpr int PA_CU = 1024;               // texts whose bounds are kept in LDS
+constexpr int PA_CU = 1023;               // texts whose bounds are kept in LDS
 
 // four consecutive dims of one (token, head) of the output
 template <class T, int HD>
@@ -214,13 +240,85 @@ __device__ __forceinline__ void prompt_store4(const PromptArgs &a, int token, in
     *reinterpret_cast<uint2 *>(p) = make_uint2(T::pack(x, y), T::pack(z, w));
 }
 
+// the kernel's arguments once more, read from memory where they are used: the epilogues' share of them would otherwise sit in scalar
+// registers all through the loop over the keys (120 of them spilled)
+__device__ __forceinline__ const PromptArgs &args_again() {
+    uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PromptArgs *)(const __attribute__((address_space(4))) PromptArgs *)p;
+}
+
+// a wave's 32 rows: O^T tiles, the maxima and this half's sums -> the output, or this split's partials.  Prompt keys [p0, p1) and own
+// keys [b0, b1) are what this workgroup went through.
+template <class T, int HD>
+__device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float mrow, float lrow, int row, int token, int head, int lo, int hi,
+                                              bool live, int split, int kvh, int64_t p0, int64_t p1, int64_t b0, int64_t b1, float *qs) {
+    constexpr int NDT = HD / 32, DPL = HD / 64;
+    const PromptArgs &a = args_again();
+    const int lane = threadIdx.x & 63, li = lane & 31, half = lane >> 5, rows = a.n_tokens * a.G;
+    const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lrow), __float_as_uint(lrow), false, false);
+    lrow = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    float zero = lrow * 0.f;                                                     // NaN if anything is no finite number
+#pragma unroll
+    for (int n = 0; n < NDT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(o[n][r], 0.f, zero);
+    uint64_t redo = __builtin_amdgcn_ballot_w64(zero != 0.f && live);
+    redo = (redo | redo >> 32) & 0xffffffffu;
+    const bool sees = a.P > 0 || hi > lo;
+    const int64_t prow = ((int64_t)split * a.n_kv + kvh) * rows;                 // this split's partials of the key head
+    if (row < rows && !(redo >> li & 1) && (live || a.zero_rest || a.splits > 1)) {
+        if (a.splits > 1) {
+            float *po = a.part_o + (prow + row) * HD + 4 * half;
+#pragma unroll
+            for (int n = 0; n < NDT; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4 *>(po + 32 * n + 8 * q) = make_float4(o[n][4 * q], o[n][4 * q + 1], o[n][4 * q + 2], o[n][4 * q + 3]);
+            if (!half) a.part_ml[prow + row] = make_float2(mrow, lrow);
+        } else {
+            const float inv = live && sees ? 1.0f / lrow : 0.f;                  // (0 x inf where every score is -inf: NaN, as 0 / 0)
+            // dims 32 n + 8 q + 4 half ..: rows of the output, or fragments (prompt_store4)
+            bf16_t *po = (a.frag ? a.frag + (((int64_t)head * (HD / 32) * a.frag_mt + (token >> 4)) * 64 + (token & 15)) * 8 : a.out + token * a.o_token + head * a.o_head) + 4 * half;
+            const int sn = a.frag ? a.frag_mt * 512 : 32, sq = a.frag ? 128 : 8;
+#pragma unroll
+            for (int n = 0; n < NDT; ++n, po += sn)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint2 v = make_uint2(T::pack(o[n][4 * q] * inv, o[n][4 * q + 1] * inv), T::pack(o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv));
+                    if (!live) v = make_uint2(0u, 0u);
+                    *reinterpret_cast<uint2 *>(po + q * sq) = v;
+                }
+        }
+    }
+    while (redo) {
+        const int i = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int tk = __builtin_amdgcn_readlane(token, i), hd_ = __builtin_amdgcn_readlane(head, i), rr = __builtin_amdgcn_readlane(row, i);
+        const int l_ = __builtin_amdgcn_readlane(lo, i), h_ = __builtin_amdgcn_readlane(hi, i);
+        float ro[DPL], m, l;
+        prompt_row<T, HD>(a, tk, hd_, min(p0, (int64_t)a.P), min(p1, (int64_t)a.P), max((int64_t)l_, b0), min((int64_t)h_, b1), qs, ro, m, l);
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) {
+            const int d = lane * DPL + e;
+            if (a.splits > 1) a.part_o[(prow + rr) * HD + d] = ro[e];
+            else if (a.frag) a.frag[((((int64_t)hd_ * (HD / 32) + d / 32) * a.frag_mt + (tk >> 4)) * 64 + (d % 32) / 8 * 16 + (tk & 15)) * 8 + d % 8] = T::down(ro[e] / l);
+            else a.out[tk * a.o_token + hd_ * a.o_head + d] = T::down(ro[e] / l);
+        }
+        if (a.splits > 1 && lane == 0) a.part_ml[prow + rr] = make_float2(m, l);
+    }
+}
+
+// Two stages of LDS, so that two workgroups share a CU and overlap each other (four stages and one workgroup a CU: 88 us instead
+// of 52 on four tokens behind 65 500, 1026 instead of 1005 on 12.7 k tokens behind 4096).
 template <class T, int HD, int NW, bool VT>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
     constexpr int KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
     constexpr int RPP = 64 / SL, PIECES = KC / RPP, PPW = PIECES / NW;            // rows of a 1-KiB piece, pieces of a K or V tile, of a wave
-    constexpr int STG = 2 * KC * HD;
+    constexpr int STG = 2 * KC * HD, NS = 2;
     static_assert(PIECES % NW == 0, "pieces divide over the waves");
-    __shared__ __attribute__((aligned(16))) bf16_t smem[2 * STG];
+    __shared__ __attribute__((aligned(16))) bf16_t smem_[NS * STG];
+    lds_t *const smem = (lds_t *)smem_;
     __shared__ int s_cu[2][PA_CU + 1];
     __shared__ float s_q[NW][HD];                                               // prompt_row's
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -230,52 +328,52 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
     const int items = a.n_kv * a.splits * a.tiles, per = (items + 7) / 8;
     const int it = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if (it >= items || (int)(blockIdx.x / 8) >= per) return;
-    const int tile = it % a.tiles, split = it / a.tiles % a.splits, kvh = it / a.tiles / a.splits;
+    const int part = quotient(it, a.tiles, a.r_tiles), kvh = quotient(part, a.splits, a.r_splits), tile = it - part * a.tiles, split = part - kvh * a.splits;
     const int rows = a.n_tokens * a.G, r0 = tile * 32 * NW;
-    // bounds of the texts
-    const bool in_lds = a.cu_q && a.n_texts <= PA_CU;
-    if (in_lds) {
-        for (int i = tid; i <= a.n_texts; i += 64 * NW) { s_cu[0][i] = a.cu_q[i]; s_cu[1][i] = a.cu_k[i]; }
-        __syncthreads();
-    }
-    const int *cq = in_lds ? s_cu[0] : a.cu_q, *ck = in_lds ? s_cu[1] : a.cu_k;
-    const int t_end = min(a.cu_q ? min(cq[a.n_texts], a.n_tokens) : a.n_tokens, (r0 + 32 * NW - 1) / a.G + 1);   // tokens of this tile that belong to texts
-    const int row = r0 + 32 * w + li, token = min(row, rows - 1) / a.G, head = kvh * a.G + min(row, rows - 1) % a.G;
-    int lo, hi, k0, k1, dummy;
-    bool live = prompt_own_range(a, cq, ck, token, lo, hi) && row < rows;
-    if (!prompt_own_range(a, cq, ck, r0 / a.G, k0, dummy) || !prompt_own_range(a, cq, ck, t_end - 1, dummy, k1)) k0 = k1 = 0;
-    if (VT) k0 &= ~7;                                                           // V^T rows are read in 16-byte pieces
-    if (k1 < k0) k1 = k0;
-    // this workgroup's share of the chunks: nP of the prompt, then the texts' own
-    const int nP = (a.P + KC - 1) / KC, n_all = nP + (k1 - k0 + KC - 1) / KC;
-    const int c0 = (int)((int64_t)n_all * split / a.splits), c1 = (int)((int64_t)n_all * (split + 1) / a.splits);
+    const int row = r0 + 32 * w + li, token = quotient(min(row, rows - 1), a.G, a.r_G), head = kvh * a.G + min(row, rows - 1) - token * a.G;
+    // this workgroup's chunks 0 .. n - 1: its share of the prompt's pages, pages p0 .. p0 + np - 1, then of the 64-key pieces of its
+    // texts' own keys [k0, k1), pieces o0 ..
+    const int nP = (a.P + KC - 1) / KC;
+    const int p0 = a.splits > 1 ? (int)((int64_t)nP * split / a.splits) : 0, np = (a.splits > 1 ? (int)((int64_t)nP * (split + 1) / a.splits) : nP) - p0;
+    int k0 = 0, k1 = 0, o0 = 0;
+    auto base_of = [&](int i) { return i < np ? (p0 + i) * KC : k0 + (o0 + i - np) * KC; };   // the chunk's first key
 
-    auto kswz = [](int key) { return SL == 16 ? key & 15 : (key & 3) | ((key >> 3) & 1) << 2; };
-    auto vswz = [](int key) { return SL == 16 ? (key & 3) * 4 : ((key >> 1) & 1) * 4; };
-    auto issue = [&](int c, int stage) {
-        bf16_t *Ks = smem + stage * STG, *Vs = Ks + KC * HD;
-        if (c < nP) {
-            const bf16_t *pg = a.pages + a.table[c] * a.page_stride + (int64_t)kvh * 2 * KC * HD;
-            const int last = min(a.P - c * KC, KC) - 1;                          // rows behind the prompt's end: its last one again (masked, and finite if the prompt is)
-#pragma unroll
-            for (int i = 0; i < PPW; ++i) {
-                const int p = w * PPW + i, key = p * RPP + lane / SL, s = lane % SL, r = min(key, last);
-                dma16(pg + r * HD + (s ^ kswz(key)) * 8, Ks + p * 512);
-                dma16(pg + KC * HD + r * HD + (s ^ vswz(key)) * 8, Vs + p * 512);
-            }
+    auto swz = [](int key) { return SL == 16 ? (key & 3) << 2 | ((key >> 2) & 3) : ((key >> 1) & 1) << 2 | ((key >> 3) & 1) << 1 | (key & 1); };
+    const bf16_t *const head_pages = a.pages + (int64_t)kvh * 2 * KC * HD;
+    int next_page = np > 0 ? __builtin_amdgcn_readfirstlane(a.table[p0]) : 0;                                   // (read a chunk ahead: its latency is not the request's)
+    auto issue = [&](int i) {
+        lds_t *Ks = smem + (i % NS) * STG, *Vs = Ks + KC * HD;
+        // the base of a chunk is uniform, a lane adds 32 bits (the host bounds the strides)
+        const bf16_t *kb, *vb;
+        unsigned kt = HD * 2, vt = HD * 2;                                        // bytes from row to row
+        int last = KC - 1;                                                       // rows behind the end: the last one again (masked, and finite if that one is)
+        const bool own = i >= np;
+        const int b = base_of(i);
+        if (!own) {
+            kb = head_pages + next_page * a.page_stride;
+            vb = kb + KC * HD;
+            next_page = __builtin_amdgcn_readfirstlane(a.table[min(p0 + i + 1, nP - 1)]);
+            last = min(last, a.P - 1 - b);
         } else {
-            const int b = k0 + (c - nP) * KC;
+            kb = a.k + b * a.k_token + kvh * a.k_head;
+            kt = (unsigned)a.k_token * 2;
+            last = min(last, k1 - 1 - b);
+            if (VT) vb = a.v + (int64_t)kvh * HD * a.v_token + b;
+            else vb = a.v + b * a.v_token + kvh * a.v_head;
+            vt = (unsigned)a.v_token * 2;
+        }
+        kb = uniform(kb);
+        vb = uniform(vb);
 #pragma unroll
-            for (int i = 0; i < PPW; ++i) {
-                const int p = w * PPW + i, key = p * RPP + lane / SL, s = lane % SL;
-                const int64_t r = min(b + key, k1 - 1);
-                dma16(a.k + r * a.k_token + kvh * a.k_head + (s ^ kswz(key)) * 8, Ks + p * 512);
-                if (VT) {                                                        // 8 dims x 64 keys
-                    const int d = p * 8 + (lane >> 3), sl = lane & 7;
-                    dma16(a.v + ((int64_t)kvh * HD + d) * a.v_token + b + (sl ^ (d & 7)) * 8, Vs + p * 512);
-                } else {
-                    dma16(a.v + r * a.v_token + kvh * a.v_head + (s ^ vswz(key)) * 8, Vs + p * 512);
-                }
+        for (int e = 0; e < PPW; ++e) {                                          // (pieces dealt round the waves: a wave's pieces differ by whole multiples of the slot pattern)
+            const int p = e * NW + w, key = p * RPP + lane / SL, r = min(key, last);
+            const unsigned slot = (unsigned)((lane % SL) ^ swz(key)) * 16;
+            dma16(kb, r * kt + slot, Ks + p * 512);
+            if (VT && own) {                                                     // 8 dims x 64 keys
+                const int d = p * 8 + (lane >> 3);
+                dma16(vb, d * vt + (unsigned)((lane & 7) ^ (d & 7)) * 16, Vs + p * 512);
+            } else {
+                dma16(vb, r * vt + slot, Vs + p * 512);
             }
         }
     };
@@ -298,172 +396,239 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
                 }
             }
         }
+    };
+    auto pin_q = [&] {                                                           // (the wait for them sits here, not in the loop, where it would drain the DMA)
 #pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[kk]));        // (the wait for them sits here, not in the loop, where it would drain the DMA)
+        for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[kk]));
     };
 
+    // The first accesses of everything, one behind the other (each is a miss of 1 - 2 us): the texts' bounds, Q, the prompt's pages,
+    // then the texts' own keys.
+    const bool in_lds = a.cu_q && a.n_texts <= PA_CU;
+    constexpr int CPT = (PA_CU + 1) / (64 * NW);                                 // bounds of a thread
+    int b_q[CPT] = {}, b_k[CPT] = {};
+    if (in_lds) {
+#pragma unroll
+        for (int e = 0; e < CPT; ++e) {
+            const int i = tid + 64 * NW * e;
+            if (i <= a.n_texts) { b_q[e] = a.cu_q[i]; b_k[e] = a.cu_k[i]; }
+        }
+    }
+    load_q(a.inter && np > 0);
+    if (in_lds) {
+#pragma unroll
+        for (int e = 0; e < CPT; ++e) {
+            const int i = tid + 64 * NW * e;
+            if (i <= a.n_texts) { s_cu[0][i] = b_q[e]; s_cu[1][i] = b_k[e]; }
+        }
+    }
+    const int early = min(np, NS);
+    for (int i = 0; i < early; ++i) issue(i);
+    if (in_lds) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int *cq = in_lds ? s_cu[0] : a.cu_q, *ck = in_lds ? s_cu[1] : a.cu_k;
+    // one search for all: lanes 0 .. 31 for their rows, lane 32 for the tile's first token, the others for the last one that belongs to a text
+    const int t_end = min(a.cu_q ? min(cq[a.n_texts], a.n_tokens) : a.n_tokens, quotient(min(r0 + 32 * NW, rows) - 1, a.G, a.r_G) + 1);
+    int lo, hi;
+    bool live = prompt_own_range(a, cq, ck, half ? (li ? t_end - 1 : quotient(r0, a.G, a.r_G)) : token, lo, hi);
+    const uint64_t found = __builtin_amdgcn_ballot_w64(live);
+    k0 = __builtin_amdgcn_readlane(lo, 32);
+    k1 = __builtin_amdgcn_readlane(hi, 33);
+    if ((found >> 32 & 3) != 3) k0 = k1 = 0;
+    lo = __builtin_amdgcn_permlane32_swap(lo, lo, false, false)[0];              // (the lower half's, in both)
+    hi = __builtin_amdgcn_permlane32_swap(hi, hi, false, false)[0];
+    live = (found >> li & 1) && row < rows;
+    const bool wave_live = __builtin_amdgcn_ballot_w64(live) != 0;
+    if (VT) k0 &= ~7;                                                           // V^T rows are read in 16-byte pieces
+    k1 = max(k1, k0);
+    const int nO = (k1 - k0 + KC - 1) / KC;
+    o0 = a.splits > 1 ? (int)((int64_t)nO * split / a.splits) : 0;
+    const int n = np + (a.splits > 1 ? (int)((int64_t)nO * (split + 1) / a.splits) : nO) - o0;
+    for (int i = early; i < min(n, NS); ++i) issue(i);
+    pin_q();
     f32x16 o[NDT];
 #pragma unroll
-    for (int n = 0; n < NDT; ++n) o[n] = (f32x16)(0.f);
+    for (int d = 0; d < NDT; ++d) o[d] = (f32x16)(0.f);
     float mrow = -__builtin_huge_valf(), lrow = 0.f;
     const int krow = (li & 0x13) | ((li & 4) << 1) | ((li & 8) >> 1);             // bits 2 and 3 exchanged
-    const int kkey = kswz(krow);
+    const int kkey = swz(krow);
     // transposing reads: lane (16 g + i) of a half addresses key 8 half + i / 4, dims 16 g + 4 (i % 4)
     const int vkey = 8 * half + ((lane & 15) >> 2), vslot = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vhalf = (lane & 1) * 4;
 
-    auto compute = [&](int c, int stage) {
-        const bf16_t *Ks = smem + stage * STG, *Vs = Ks + KC * HD;
-        const bool own = c >= nP;
-        const int b = own ? k0 + (c - nP) * KC : c * KC;
-        // keys [l, h) of the chunk are this row's
-        const int l = own ? max(lo - b, 0) : 0, h = !live ? 0 : min(own ? hi - b : a.P - b, KC);
-        if (!__builtin_amdgcn_ballot_w64(l < h)) return;                        // (a wave none of whose rows sees the chunk)
+    // what this wave has to do with chunk i: nothing, the plain product, or with a mask
+    enum { SKIP = 0, FULL = 1, MASK = 2 };
+    auto mode = [&](int i) {
+        const int b = base_of(i);
+        if (i < np) return !wave_live ? SKIP : b + KC <= a.P ? FULL : MASK;
+        if (!__builtin_amdgcn_ballot_w64(live && lo < b + KC && hi > b)) return SKIP;
+        return __builtin_amdgcn_ballot_w64(live && (lo > b || hi < b + KC)) ? MASK : FULL;
+    };
+    // A chunk is two tiles of 32 keys, each with its own online-softmax step, so that matrix and vector work of one wave overlap:
+    //   S0 = K0 Q^T | S1 = K1 Q^T beside the exponentials of S0 | O += V0^T P0 beside those of S1 | O += V1^T P1
+    // sched_barrier keeps the slots (a product, its share of the exponentials, the LDS reads of four products later) as written.
+    auto product = [&](int i, int md) {
+        const lds_t *Ks = smem + (i % NS) * STG, *Vs = Ks + KC * HD;
+        constexpr int EPS = 16 / NKK;                                            // exponentials of a slot (both phases have NKK slots a tile)
+        static_assert(2 * NDT == NKK, "as many products of V as of K");
+        u32x4 kf[4], vf[4], pf[4];                                               // fragments in flight; probabilities, packed: keys 16 J + 8 half ..
         f32x16 s[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            s[j] = (f32x16)(0.f);
-            const bf16_t *kb = Ks + (32 * j + krow) * HD;
-#pragma unroll
-            for (int kk = 0; kk < NKK; ++kk) s[j] = T::mfma(*reinterpret_cast<const u32x4 *>(kb + (((2 * kk + half) ^ kkey) * 8)), qf[kk], s[j]);
-        }
-        if (__builtin_amdgcn_ballot_w64(l > 0 || h < KC)) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
+        const bool own = i >= np;
+        const int b = base_of(i), l = own ? lo - b : 0, h = (own ? hi : a.P) - b;   // the row sees keys [l, h) of the chunk
+        auto read_k = [&](int f) { kf[f & 3] = lds_16(Ks + (krow + 32 * (f / NKK)) * HD + (((2 * (f % NKK) + half) ^ kkey) * 8)); };
+        auto read_v = [&](int g) {
+            const int J = g / NDT, n = g % NDT;
+            if (VT && own) {
+                vf[g & 3] = lds_16(Vs + (32 * n + li) * KC + (((2 * J + half) ^ (li & 7)) * 8));
+            } else {
+                const lds_t *vp = Vs + (16 * J + vkey) * HD + vhalf;
+                const u32x2 x = lds_tr(vp + ((4 * n + vslot) ^ swz(vkey)) * 8), y = lds_tr(vp + 4 * HD + ((4 * n + vslot) ^ swz(vkey + 4)) * 8);
+                vf[g & 3] = (u32x4){x[0], x[1], y[0], y[1]};
+            }
+        };
+        float sub = 0.f, sum[2] = {0.f, 0.f};
+        auto top = [&](auto J_) {                                                // mask, and the row's maximum
+            constexpr int j = decltype(J_)::value;
+            if (md == MASK) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int key = 32 * j + 16 * (r >> 3) + 8 * half + (r & 7);
                     if (key < l || key >= h) s[j][r] = -__builtin_huge_valf();
                 }
-        }
-        float mx = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
-        const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale2;
-        if (__builtin_amdgcn_ballot_w64(mx > mrow + 8.f)) {
-            const float mn = fmaxf(mrow, mx);
-            const float alpha = mrow == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(mrow - mn);
-            mrow = mn;
-            lrow *= alpha;
-#pragma unroll
-            for (int n = 0; n < NDT; ++n) o[n] *= alpha;
-        }
-        const float sub = (mrow == -__builtin_huge_valf() ? 0.f : mrow) - T::shift;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], a.scale2, -sub));
-                lrow += s[j][r];
             }
+            float mx = s[j][0];
 #pragma unroll
-        for (int J = 0; J < 4; ++J) {
-            u32x4 pf;
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+            const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale2;
+            if (__builtin_amdgcn_ballot_w64(mx > mrow + 8.f)) {
+                const float mn = fmaxf(mrow, ceilf(mx));                          // (whole numbers: the factor is a power of two, exact on what is rounded already)
+                const float alpha = mrow == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(mrow - mn);
+                mrow = mn;
+                lrow *= alpha;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pf[e] = T::pack(s[J >> 1][8 * (J & 1) + 2 * e], s[J >> 1][8 * (J & 1) + 2 * e + 1]);
+                for (int n = 0; n < NDT; ++n) o[n] *= alpha;
+                if constexpr (j == 1) {
+                    sum[0] *= alpha;
+                    sum[1] *= alpha;
 #pragma unroll
-            for (int n = 0; n < NDT; ++n) {
-                u32x4 vf;
-                if (VT && own) {
-                    vf = *reinterpret_cast<const u32x4 *>(Vs + (32 * n + li) * KC + (((2 * J + half) ^ (li & 7)) * 8));
-                } else {
-                    const bf16_t *vp = Vs + (16 * J + vkey) * HD + vhalf;
-                    const u32x2 x = lds_tr(vp + ((4 * n + vslot) ^ vswz(vkey)) * 8), y = lds_tr(vp + 4 * HD + ((4 * n + vslot) ^ vswz(vkey + 4)) * 8);
-                    vf = (u32x4){x[0], x[1], y[0], y[1]};
+                    for (int q = 0; q < 2; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            pf[q][e] = T::pack(T::up((unsigned short)(pf[q][e] & 0xffffu)) * alpha, T::up((unsigned short)(pf[q][e] >> 16)) * alpha);
                 }
-                o[n] = T::mfma(vf, pf, o[n]);
             }
+            sub = (mrow == -__builtin_huge_valf() ? 0.f : mrow) - T::shift;
+        };
+        auto exps = [&](auto J_, int slot) {                                     // EPS of tile j's probabilities
+            constexpr int j = decltype(J_)::value;
+#pragma unroll
+            for (int e = 0; e < EPS; ++e) {
+                const int r = slot * EPS + e;
+                s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], a.scale2, -sub));
+                sum[e & 1] += s[j][r];
+                if (r & 1) {
+                    unsigned two = T::pack(s[j][r - 1], s[j][r]);
+                    asm volatile("" : "+v"(two), "+v"(sum[0]), "+v"(sum[1]));    // (here, not where it is used: the compiler sinks it past the products)
+                    pf[2 * j + r / 8][r / 2 % 4] = two;
+                }
+            }
+        };
+        s[0] = s[1] = (f32x16)(0.f);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) read_k(f);
+#pragma unroll
+        for (int f = 0; f < NKK; ++f) {
+            s[0] = T::mfma(kf[f & 3], qf[f], s[0]);
+            read_k(f + 4);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        top(std::integral_constant<int, 0>{});
+#pragma unroll
+        for (int f = 0; f < NKK; ++f) {
+            s[1] = T::mfma(kf[f & 3], qf[f], s[1]);
+            if (f + 4 < NKK) read_k(NKK + f + 4);
+            else read_v(f + 4 - NKK);
+            exps(std::integral_constant<int, 0>{}, f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        top(std::integral_constant<int, 1>{});
+#pragma unroll
+        for (int g = 0; g < NKK; ++g) {
+            o[g % NDT] = T::mfma(vf[g & 3], pf[g / NDT], o[g % NDT]);
+            read_v(g + 4);
+            exps(std::integral_constant<int, 1>{}, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        lrow += sum[0] + sum[1];
+#pragma unroll
+        for (int g = NKK; g < 2 * NKK; ++g) {
+            o[g % NDT] = T::mfma(vf[g & 3], pf[g / NDT], o[g % NDT]);
+            if (g + 4 < 2 * NKK) read_v(g + 4);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
+    auto landed = [&](int later) {                                               // own pieces of all but the last `later` chunks requested
+        if (later) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PPW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
 
-    if (c0 < c1) {
-        load_q(a.inter && c0 < nP);
-        issue(c0, 0);
-        for (int c = c0; c < c1; ++c) {
-            if (a.inter && c == nP && c > c0) load_q(false);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // own pieces of chunk c
-            __syncthreads();                                                     // everyone's; chunk c - 1 is used up
-            if (c + 1 < c1) issue(c + 1, (c + 1 - c0) & 1);
-            compute(c, (c - c0) & 1);
-        }
+    for (int i = 0; i < n; ++i) {
+        if (a.inter && i == np && i > 0) { load_q(false); pin_q(); }
+        landed(i == 0 && n > 1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");             // everyone's pieces; the chunk before is used up
+        if (i > 0 && i + 1 < n) issue(i + 1);
+        const int md = mode(i);
+        if (md != SKIP) product(i, md);
     }
-
-    {
-        const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lrow), __float_as_uint(lrow), false, false);
-        lrow = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-    }
-    bool bad = not_finite(lrow);
-#pragma unroll
-    for (int n = 0; n < NDT; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bad = bad || not_finite(o[n][r]);
-    uint64_t redo = __builtin_amdgcn_ballot_w64(bad && live);
-    redo = (redo | redo >> 32) & 0xffffffffu;
-    const bool sees = a.P > 0 || hi > lo;
-    const int64_t prow = ((int64_t)split * a.n_kv + kvh) * rows;                 // this split's partials of the key head
-    if (row < rows && !(redo >> li & 1) && (live || a.zero_rest || a.splits > 1)) {
-        if (a.splits > 1) {
-            float *po = a.part_o + (prow + row) * HD;
-#pragma unroll
-            for (int n = 0; n < NDT; ++n)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<float4 *>(po + 32 * n + 8 * q + 4 * half) = make_float4(o[n][4 * q], o[n][4 * q + 1], o[n][4 * q + 2], o[n][4 * q + 3]);
-            if (!half) a.part_ml[prow + row] = make_float2(mrow, lrow);
-        } else {
-            const float inv = live && sees ? 1.0f / lrow : 0.f;                  // (0 x inf where every score is -inf: NaN, as 0 / 0)
-#pragma unroll
-            for (int n = 0; n < NDT; ++n)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    prompt_store4<T, HD>(a, token, head, 32 * n + 8 * q + 4 * half, o[n][4 * q] * inv, o[n][4 * q + 1] * inv, o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv);
-        }
-    }
-    while (redo) {
-        const int i = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        const int tk = __builtin_amdgcn_readlane(token, i), hd_ = __builtin_amdgcn_readlane(head, i), rr = __builtin_amdgcn_readlane(row, i);
-        const int l_ = __builtin_amdgcn_readlane(lo, i), h_ = __builtin_amdgcn_readlane(hi, i);
-        constexpr int DPL = HD / 64;
-        float ro[DPL], m, l;
-        const int64_t b0 = (int64_t)k0 + (int64_t)max(c0 - nP, 0) * KC, b1 = (int64_t)k0 + (int64_t)max(c1 - nP, 0) * KC;   // own keys of this split
-        prompt_row<T, HD>(a, tk, hd_, min((int64_t)c0 * KC, (int64_t)a.P), min((int64_t)c1 * KC, (int64_t)a.P), max((int64_t)l_, b0), min((int64_t)h_, b1), s_q[w], ro, m, l);
-#pragma unroll
-        for (int e = 0; e < DPL; ++e) {
-            const int d = lane * DPL + e;
-            if (a.splits > 1) a.part_o[(prow + rr) * HD + d] = ro[e];
-            else if (a.frag) a.frag[((((int64_t)hd_ * (HD / 32) + d / 32) * a.frag_mt + (tk >> 4)) * 64 + (d % 32) / 8 * 16 + (tk & 15)) * 8 + d % 8] = T::down(ro[e] / l);
-            else a.out[tk * a.o_token + hd_ * a.o_head + d] = T::down(ro[e] / l);
-        }
-        if (a.splits > 1 && lane == 0) a.part_ml[prow + rr] = make_float2(m, l);
-    }
+    prompt_finish<T, HD>(o, mrow, lrow, row, token, head, lo, hi, live, split, kvh, (int64_t)p0 * KC, (int64_t)(p0 + np) * KC,
+                         (int64_t)k0 + (int64_t)o0 * KC, (int64_t)k0 + (int64_t)(o0 + n - np) * KC, s_q[w]);
 }
 
-// the splits' partials of a row -> the output: a wave per row, o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the splits' order
-template <class T, int HD>
+// the splits' partials of a row -> the output: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  HD / 4 lanes hold four dims each; PAR
+// such groups take every PAR-th split of a row (8 where there are more than 8 splits: one group would go through them as one chain
+// of loads, 34 us at 64 splits) and meet in LDS, always in the same order.
+template <class T, int HD, int PAR>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
-    constexpr int LPR = HD / 4;                                                  // lanes of a row, four dims each
-    const int rows = a.n_tokens * a.G;
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
-    if (i >= (int64_t)rows * a.n_kv) return;
-    const int d = threadIdx.x % LPR * 4, kvh = (int)(i / rows), row = (int)(i % rows), token = row / a.G, head = kvh * a.G + row % a.G;
+    constexpr int LPR = HD / 4, RPB = 256 / LPR / PAR;                           // lanes of a group, rows of a workgroup
+    __shared__ float4 s_o[PAR][RPB][LPR];
+    __shared__ float2 s_ml[PAR][RPB];
+    const int rows = a.n_tokens * a.G, g = threadIdx.x / LPR % PAR, rb = threadIdx.x / LPR / PAR, ln = threadIdx.x % LPR;
+    const int64_t n = (int64_t)rows * a.n_kv, i = (int64_t)blockIdx.x * RPB + rb, at = i < n ? i : n - 1;
+    float m = -__builtin_huge_valf(), l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 x) {                                        // (a split that saw no key of the row has zeros and the maximum -inf)
+        const float mn = fmaxf(m, ml.x), sub = mn == -__builtin_huge_valf() ? 0.f : mn;
+        const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - sub), e = ml.x == -__builtin_huge_valf() && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - sub);
+        m = mn;
+        l = l * f + e * ml.y;
+        o.x = o.x * f + e * x.x; o.y = o.y * f + e * x.y; o.z = o.z * f + e * x.z; o.w = o.w * f + e * x.w;
+    };
+    constexpr int U = 8;                                                          // partials in flight
+    for (int s0 = g; s0 < a.splits; s0 += U * PAR) {
+        float2 ml[U];
+        float4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t s = min(s0 + u * PAR, a.splits - 1);
+            ml[u] = a.part_ml[s * n + at];
+            x[u] = *reinterpret_cast<const float4 *>(a.part_o + (s * n + at) * HD + ln * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * PAR < a.splits) add(ml[u], x[u]);
+    }
+    if constexpr (PAR > 1) {
+        s_o[g][rb][ln] = o;
+        if (ln == 0) s_ml[g][rb] = make_float2(m, l);
+        __syncthreads();
+        if (g) return;
+        for (int q = 1; q < PAR; ++q) add(s_ml[q][rb], s_o[q][rb][ln]);
+    }
+    if (i >= n) return;
+    const int d = ln * 4, kvh = (int)(i / rows), row = (int)(i % rows), token = row / a.G, head = kvh * a.G + row % a.G;
     int lo, hi;
     const bool live = prompt_own_range(a, a.cu_q, a.cu_k, token, lo, hi);
     if (!live && !a.zero_rest) return;
-    float m = -__builtin_huge_valf(), l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int64_t n = (int64_t)rows * a.n_kv;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * n + i].x);
-    const float sub = m == -__builtin_huge_valf() ? 0.f : m;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * n + i];
-        const float4 x = *reinterpret_cast<const float4 *>(a.part_o + (s * n + i) * HD + d);
-        const float f = __builtin_amdgcn_exp2f(ml.x - sub);
-        l += f * ml.y;
-        // (a split that saw no key of the row has zeros; its weight is 0 too)
-        o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
-    }
-    const float inv = live && (a.P > 0 || hi > lo) ? 1.0f / l : 0.f;
+    const float inv = a.P > 0 || hi > lo ? 1.0f / l : 0.f;
     if (live) prompt_store4<T, HD>(a, token, head, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     else prompt_store4<T, HD>(a, token, head, d, 0.f, 0.f, 0.f, 0.f);
 }
