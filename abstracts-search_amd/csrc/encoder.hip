@@ -17,6 +17,7 @@
 #include "encoder_kernels.h"
 #include "encoder_few.h"
 #include "encoder_mid.h"
+#include "prompt_cache.h"
 
 using namespace mi;
 using namespace mienc;
@@ -112,6 +113,7 @@ std::atomic<int64_t> g_mid_launches{0};   // QKV / O projections on the one-laun
 std::atomic<int64_t> g_few_passes{0};     // forward passes that took the query-time path (encoder_few.h)
 std::atomic<int64_t> g_few_qkv8_passes{0}; // ... with the QKV projection's fragments in registers (few_qkv8_kernel)
 std::atomic<int64_t> g_few_gu8_passes{0}; // ... with the gate/up projection on 8-feature units (few_gu8_kernel)
+std::atomic<int64_t> g_prompted_passes{0}; // forward passes behind a cached prompt (mi_encoder_encode_prompted, mi_encoder_cache_prompt)
 std::atomic<int64_t> g_few_ao_passes{0};  // ... of them, with the attention inside the O projection (few_ao_kernel)
 
 struct LayerW {
@@ -696,6 +698,7 @@ struct mi_encoder {
     };
     struct WS {
         std::mutex mu;
+        DevBuf ws_prompt;        // partials of the prompted attention
         DevBuf ws_x, ws_xn, ws_qk, ws_vt, ws_att, ws_h, ws_up, ws_out, ws_stage, ws_part, ws_ssq, ws_arrive, few_ctr, ws_skpart, ws_skctr;
         Pinned pin[3];
         int pin_next = 0;
@@ -712,6 +715,34 @@ struct mi_encoder {
     // profiling: the GEMM launches of the most recent encode (arguments as launched), replayed back to back between two
     // HIP events by mi_encoder_profile_read -- like the index library's scan replay; per-launch event pairs measured
     // 3-4 % short of rocprofv3's per-kernel durations in the same run
+    // cached prompts (causal models): their keys and values live in one pool of pages, the sum of their final hidden states beside
+    // them.  A pass holds a reference, so that a prompt dropped meanwhile goes when the pass has been issued.
+    struct Prompt {
+        mi_prompt_cache *cache = nullptr;
+        int32_t entry = -1;
+        void *stream = nullptr;              // it was made on
+        int device = 0;
+        std::vector<int32_t> ids;
+        DevBuf sum;                          // f32 [hidden]: the tokens' final-norm hidden states (bf16 values, as the pooling sees them)
+        ~Prompt() {
+            if (entry < 0) return;
+            int prev = 0;
+            (void)hipGetDevice(&prev);
+            (void)hipSetDevice(device);
+            (void)mi_prompt_cache_free(cache, 1, &entry, stream);
+            sum.release();
+            (void)hipSetDevice(prev);
+        }
+    };
+    std::mutex prompts_mu;                   // guards the two below, and one mi_encoder_cache_prompt at a time
+    mi_prompt_cache *prompt_cache = nullptr;
+    std::map<int32_t, std::shared_ptr<Prompt>> prompts;
+    int32_t next_prompt = 0;
+    int prompt_pages = 0;                    // of the pool
+    ~mi_encoder() {
+        prompts.clear();
+        if (prompt_cache) (void)mi_prompt_cache_destroy(prompt_cache);
+    }
     bool prof = false;
     struct Launch { int epi; GemmArgs g; };
     std::vector<Launch> prof_launches;
@@ -780,14 +811,21 @@ struct Batch {
     int nseq = 0, T_real = 0, T_pad = 0, Lmax = 0, nwork = 0;
     // device pointers into ws_up
     int32_t *ids = nullptr, *pos = nullptr;
+    // a batch behind a cached prompt: the prompt's entry and the tokens of it that the batch sees, and where this pass's own keys and
+    // values go (store >= 0: mi_encoder_cache_prompt)
+    std::shared_ptr<mi_encoder::Prompt> prompt;
+    int prompt_len = 0;
+    int32_t store = -1;
+    bool prompted = false;
     int32_t *seq_start = nullptr, *seq_len = nullptr, *work_seq = nullptr, *work_q0 = nullptr, *tok_map = nullptr, *out_rows = nullptr;
 };
 
 // Build the packed layout (sequences back to back, T_pad = the total rounded up to a multiple of 32) straight into a
 // pinned staging slot and upload ids / positions / work lists (/ output rows) with one asynchronous copy.  Host `ids` /
 // `cu_seqlens` / `out_rows` are consumed before the call returns; nothing here waits for the GPU.
+// pos0: the position of every sequence's first token (the length of a cached prompt in front of it).
 Batch prepare_batch(mi_encoder *h, mi_encoder::WS &ws, int nseq, const int32_t *ids, const int32_t *cu, const int32_t *out_rows,
-                    hipStream_t st) {
+                    hipStream_t st, int pos0 = 0) {
     MI_REQUIRE(nseq > 0, "encode: nseq must be positive");
     std::vector<int32_t> cu_dev, ids_dev;                 // device-resident inputs (rare): fetched, which does synchronise
     if (is_device_ptr(cu)) {
@@ -810,14 +848,14 @@ Batch prepare_batch(mi_encoder *h, mi_encoder::WS &ws, int nseq, const int32_t *
     for (int i = 0; i < nseq; ++i) {
         const int L = cu[i + 1] - cu[i];
         MI_REQUIRE(L >= 1, "encode: empty sequence");
-        MI_REQUIRE(L <= h->cfg.max_seq_len, "encode: sequence longer than max_seq_len");
+        MI_REQUIRE(L <= h->cfg.max_seq_len - pos0, "encode: sequence longer than max_seq_len");
         b.Lmax = std::max(b.Lmax, L);
         nwork += (L + 63) / 64;
         cur += L;                 // back to back: the attention kernel masks the < 8 foreign keys in front of a sequence
     }
     b.T_pad = (cur + 31) & ~31;   // GEMM rows are clamped / guarded, no tile multiple needed
     b.nwork = nwork;
-    const size_t n_up = (size_t)b.T_pad * 2 + (size_t)nseq * 3 + (size_t)nwork * 2 + (size_t)T_real;
+    const size_t n_up = (size_t)b.T_pad * 2 + (size_t)nseq * 3 + 1 + (size_t)nwork * 2 + (size_t)T_real;
     mi_encoder::Pinned &pin = ws.pin[ws.pin_next];
     ws.pin_next = (ws.pin_next + 1) % 3;
     if (pin.in_flight) {                                  // (three calls ago: long consumed unless the stream is that far behind)
@@ -831,7 +869,7 @@ Batch prepare_batch(mi_encoder *h, mi_encoder::WS &ws, int nseq, const int32_t *
         pin.cap = n_up + n_up / 4 + 1024;
         MI_HIP(hipHostMalloc(reinterpret_cast<void **>(&pin.p), pin.cap * 4, hipHostMallocDefault));
     }
-    int32_t *ids_pad = pin.p, *pos = ids_pad + b.T_pad, *start = pos + b.T_pad, *len = start + nseq, *wseq = len + nseq,
+    int32_t *ids_pad = pin.p, *pos = ids_pad + b.T_pad, *start = pos + b.T_pad, *len = start + nseq + 1, *wseq = len + nseq,
             *wq0 = wseq + nwork, *tok_map = wq0 + nwork, *rows = tok_map + T_real;
     std::memset(ids_pad, 0, (size_t)b.T_pad * 8);         // ids and positions of the padding tokens
     cur = 0;
@@ -850,11 +888,12 @@ Batch prepare_batch(mi_encoder *h, mi_encoder::WS &ws, int nseq, const int32_t *
             const int32_t id = ids[(size_t)c0 + t];
             MI_REQUIRE(id >= 0 && id < vocab, "encode: token id out of range");
             ids_pad[(size_t)cur + t] = id;
-            pos[(size_t)cur + t] = t;
+            pos[(size_t)cur + t] = pos0 + t;
             tok_map[(size_t)c0 + t] = cur + t;
         }
         cur += L;
     }
+    start[nseq] = cur;                                    // (seq_start is the cumulative array of the packed lengths)
     int32_t *d = ws.ws_up.as<int32_t>(n_up);
     MI_HIP(hipMemcpyAsync(d, pin.p, n_up * 4, hipMemcpyHostToDevice, st));
     MI_HIP(hipEventRecord(pin.ev, st));
@@ -862,7 +901,7 @@ Batch prepare_batch(mi_encoder *h, mi_encoder::WS &ws, int nseq, const int32_t *
     b.ids = d;
     b.pos = d + b.T_pad;
     b.seq_start = b.pos + b.T_pad;
-    b.seq_len = b.seq_start + nseq;
+    b.seq_len = b.seq_start + nseq + 1;
     b.work_seq = b.seq_len + nseq;
     b.work_q0 = b.work_seq + nwork;
     b.tok_map = b.work_q0 + nwork;
@@ -920,6 +959,27 @@ int timed_gemm(mi_encoder *h, int epi, const GemmArgs &g, hipStream_t st) {
     h->prof_stream = st;
     h->prof_flops += 2.0 * (double)g.M * (double)g.N * (double)g.K;
     return normed;
+}
+
+// the attention of a batch behind a cached prompt, layer `layer`; a pass that stores its own keys and values (mi_encoder_cache_prompt)
+// does so first.  inter: Q and K have their rotary pairs interleaved (the fused QKV epilogues); the pages hold the weights' order.
+void launch_prompted(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, int layer, const bf16_t *qk, const bf16_t *vt, bf16_t *att, int ldvt, bool inter,
+                     hipStream_t st, bf16_t *att_frag = nullptr, int frag_mt = 0) {
+    const mi_encoder_cfg &c = h->cfg;
+    const int hd = c.head_dim;
+    const bf16_t *k = qk + (size_t)c.n_heads * hd;
+    if (b.store >= 0) prompt_cache_write_vt(h->prompt_cache, b.store, layer, b.prompt_len, b.T_real, k, h->qk_cols, inter, vt, ldvt, st);
+    mi_prompt_attn a{};
+    a.entry = b.prompt ? b.prompt->entry : b.store; a.layer = layer; a.n_heads = c.n_heads;
+    a.n_tokens = a.n_keys = b.T_real; a.n_texts = b.nseq;
+    a.q = qk; a.k = k; a.v = vt; a.out = att_frag ? att_frag : att;
+    a.q_token = a.k_token = h->qk_cols; a.q_head = a.k_head = hd; a.v_token = ldvt; a.o_token = h->q_cols; a.o_head = hd;
+    a.cu_q = a.cu_k = b.seq_start; a.causal = 1; a.scale = 1.0f / std::sqrt((float)hd);
+    PromptForms f;
+    f.vt = true; f.inter = inter; f.frag = att_frag; f.frag_mt = frag_mt; f.prompt_tokens = b.prompt_len;
+    const int64_t bytes = prompt_attention_workspace(h->prompt_cache, a);
+    if (bytes) { a.workspace = ws.ws_prompt.reserve((size_t)bytes); a.workspace_bytes = bytes; }
+    prompt_attention(h->prompt_cache, a, f, st);
 }
 
 void launch_attention(mi_encoder *h, const Batch &b, const bf16_t *qk, const bf16_t *vt, bf16_t *att, int ldvt, hipStream_t st,
@@ -1088,7 +1148,7 @@ void few_stack(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, float *x, bf16
     // one sequence of <= 32 tokens (the prompted query): the attention runs inside the O projection's workgroups (few_ao_kernel),
     // its operands arrive from the QKV epilogue as pieces (they fit the row buffers: T_pad >= 16 MT)
     const size_t ao_lds = ((size_t)c.n_kv_heads * (2 * (c.head_dim / 32) + c.head_dim / 16) + (size_t)FEW_AW * MT) * 1024;
-    const bool fuse_ao = MT <= 2 && b.nseq == 1 && !knobs().no_few_ao && (c.head_dim == 64 || c.head_dim == 128) &&
+    const bool fuse_ao = MT <= 2 && b.nseq == 1 && !b.prompted && !knobs().no_few_ao && (c.head_dim == 64 || c.head_dim == 128) &&
                          h->q_cols == c.n_heads * c.head_dim && h->v_cols == c.n_kv_heads * c.head_dim &&
                          h->qk_cols == (c.n_heads + c.n_kv_heads) * c.head_dim && c.n_heads % std::max(c.n_kv_heads, 1) == 0 &&
                          T_pad >= 16 * MT && ldvt >= 16 * MT && ao_lds <= 64 * 1024;
@@ -1129,6 +1189,8 @@ void few_stack(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, float *x, bf16
                 else hipLaunchKernelGGL((few_ao_kernel<64, MT>), dim3((unsigned)o.nunits), dim3(64 * FEW_AW), ao_lds, st, o);
                 chk("attention + o");
             }
+        } else if (b.prompted) {
+            launch_prompted(h, ws, b, l, qk, vt, nullptr, ldvt, false, st, afrag, MT);
         } else if (b.Lmax > FEW_MAX_T || (c.head_dim != 64 && c.head_dim != 128)) {
             launch_attention(h, b, qk, vt, nullptr, ldvt, st, afrag, MT);
         } else {
@@ -1195,6 +1257,7 @@ void few_stack(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, float *x, bf16
 // returns the token tiles (1..3) of a pass that took the query-time path -- its final-norm fragments are in ws_xn --, else 0
 int run_stack(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, hipStream_t st) {
     const mi_encoder_cfg &c = h->cfg;
+    if (b.prompted) ++g_prompted_passes;
     for (auto &kv : h->loaded) MI_REQUIRE(kv.second, std::string("encoder parameter not loaded: ") + kv.first);
     const int H = c.hidden, I = c.intermediate, T = b.T_pad, hd = c.head_dim;
     const int ldvt = T + 64;
@@ -1359,7 +1422,8 @@ int run_stack(mi_encoder *h, mi_encoder::WS &ws, const Batch &b, hipStream_t st)
                                nh_qk, hd, b.pos, h->rope_cos.get<float>(),
                                h->rope_sin.get<float>(), T);
         }
-        launch_attention(h, b, qk, vt, att, ldvt, st);
+        if (b.prompted) launch_prompted(h, ws, b, l, qk, vt, att, ldvt, rope_fused, st);
+        else launch_attention(h, b, qk, vt, att, ldvt, st);
         GemmArgs o{};
         o.A = att; o.lda = h->q_cols; o.W = w.wo.get<bf16_t>(); o.ldw = h->q_cols; o.M = T; o.N = H; o.K = h->q_cols;
         o.X = x; o.ldc = H; o.part = part; o.part_bytes = part_bytes;
@@ -1473,7 +1537,11 @@ int mi_encoder_load_tensor(mi_encoder *h, const char *name_c, const void *data, 
     return guard([&] {
         MI_REQUIRE(h && name_c && data && shape, "null argument");
         MI_REQUIRE(dtype >= 0 && dtype <= 2, "bad dtype");
-        h->tiled_ok = false;   // any new weight invalidates the fragment-major copies
+        {
+            std::lock_guard<std::mutex> pl(h->prompts_mu);
+            h->prompts.clear();   // any new weight invalidates the cached prompts
+        }
+        h->tiled_ok = false;   // .. and the fragment-major copies
         h->few_ok = false;
         h->roped_ok = false;
         std::string name(name_c);
@@ -1551,7 +1619,7 @@ namespace {
 // out_rows != null: embedding i goes to row out_rows[i] of `out` (device pointer) -- the caller's un-sort, done by the
 // last kernel of the call instead of an indexing pass behind it
 void encode_impl(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu, int normalize, float *out,
-                 const int32_t *out_rows, void *stream) {
+                 const int32_t *out_rows, void *stream, const std::shared_ptr<mi_encoder::Prompt> &prompt = nullptr) {
     {
         MI_REQUIRE(h && ids && cu && out, "null argument");
         DeviceGuard dg(h->device);
@@ -1560,7 +1628,10 @@ void encode_impl(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu,
         mi_encoder::WS &ws = lease.w;
         const bool od_dev = is_device_ptr(out);
         MI_REQUIRE(!out_rows || od_dev, "encode: out_rows needs a device output");
-        Batch b = prepare_batch(h, ws, nseq, ids, cu, out_rows, st);
+        const int prompt_len = prompt ? (int)prompt->ids.size() : 0;
+        const float *prompt_sum = prompt ? prompt->sum.get<float>() : nullptr;
+        Batch b = prepare_batch(h, ws, nseq, ids, cu, out_rows, st, prompt_len);
+        if (prompt) { b.prompt = prompt; b.prompt_len = prompt_len; b.prompted = true; }
         const int few_mt = run_stack(h, ws, b, st);
         Range pool_range("mi_encoder:pool+dense+normalise");
         const mi_encoder_cfg &c = h->cfg;
@@ -1572,7 +1643,7 @@ void encode_impl(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu,
             p.xfrag = ws.ws_xn.get<bf16_t>(); p.MT = few_mt; p.H = c.hidden; p.out_dim = od;
             p.parts = std::max(1, std::min(od / 16, 256 / std::max(1, nseq)));
             p.seq_start = b.seq_start; p.seq_len = b.seq_len; p.dense_w = h->dense_w.get<bf16_t>(); p.dense_b = h->dense_b.get<float>();
-            p.raw = raw;
+            p.raw = raw; p.prompt_sum = prompt_sum; p.prompt_len = prompt_len;
             hipLaunchKernelGGL(few_pool_kernel, dim3((unsigned)nseq, (unsigned)p.parts), dim3(256), 0, st, p);
             MI_HIP(hipGetLastError());
             hipLaunchKernelGGL(few_finish_kernel, dim3((unsigned)nseq), dim3(256), 0, st, raw, od, normalize, out_rows ? b.out_rows : nullptr, out);
@@ -1594,7 +1665,7 @@ void encode_impl(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu,
         p.dense_w = c.dense_out ? h->dense_w.get<bf16_t>() : nullptr;
         p.dense_b = c.dense_out ? h->dense_b.get<float>() : nullptr;
         p.seq_start = b.seq_start; p.seq_len = b.seq_len; p.out = o; p.H = c.hidden; p.out_dim = od;
-        p.Lmax = b.Lmax; p.normalize = normalize; p.eps = c.rms_eps;
+        p.Lmax = b.Lmax; p.normalize = normalize; p.eps = c.rms_eps; p.prompt_sum = prompt_sum; p.prompt_len = prompt_len;
         const size_t smem = ((size_t)b.Lmax + c.hidden + od + 8) * 4;
         // many sequences: final RMSNorm over all tokens (one wave per token, HBM speed), a mean-pool kernel, then Dense
         // as ONE GEMM over all sequences -- the pooled vectors as its bf16 A operand, residual epilogue on a zeroed
@@ -1609,7 +1680,7 @@ void encode_impl(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu,
                                c.rms_eps, xn);
             MI_HIP(hipGetLastError());
             bf16_t *pb = ws.ws_stage.as<bf16_t>((size_t)nseq * H);
-            hipLaunchKernelGGL(meanpool_kernel, dim3(nseq, (H + 511) / 512), dim3(256), 0, st, xn, b.seq_start, b.seq_len, H, pb);
+            hipLaunchKernelGGL(meanpool_kernel, dim3(nseq, (H + 511) / 512), dim3(256), 0, st, xn, b.seq_start, b.seq_len, H, pb, prompt_sum, prompt_len);
             MI_HIP(hipGetLastError());
             MI_HIP(hipMemsetAsync(o, 0, (size_t)nseq * od * 4, st));
             GemmArgs g{};
@@ -1651,6 +1722,104 @@ int mi_encoder_encode_rows(mi_encoder *h, int nseq, const int32_t *ids, const in
         MI_REQUIRE(out_rows, "null argument");
         MI_REQUIRE(!is_device_ptr(out_rows), "mi_encoder_encode_rows: out_rows is a host array");
         encode_impl(h, nseq, ids, cu, normalize, out, out_rows, stream);
+    });
+}
+
+int mi_encoder_cache_prompt(mi_encoder *h, int n, const int32_t *ids, int32_t *prompt, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(h && ids && prompt, "null argument");
+        MI_REQUIRE(!is_device_ptr(ids), "mi_encoder_cache_prompt: ids is a host array");
+        const mi_encoder_cfg &c = h->cfg;
+        MI_REQUIRE(c.causal, "cached prompts need a causal model: in a bidirectional one a prompt's hidden states depend on the text behind it");
+        MI_REQUIRE(n >= 1 && n < c.max_seq_len, "a cached prompt holds 1 .. max_seq_len - 1 tokens");
+        DeviceGuard dg(h->device);
+        hipStream_t st = as_stream(stream);
+        std::lock_guard<std::mutex> pl(h->prompts_mu);
+        constexpr int max_prompts = 256;
+        MI_REQUIRE(h->prompts.size() < max_prompts, "more than 256 cached prompts");
+        for (int i = 0; i < n; ++i) MI_REQUIRE(ids[i] >= 0 && ids[i] < c.vocab_size, "encode: token id out of range");
+        // the longest cached prompt that this one begins with: its pages are shared, only the tokens behind it are run
+        std::shared_ptr<mi_encoder::Prompt> base;
+        for (auto &kv : h->prompts) {
+            const auto &q = kv.second;
+            if ((int)q->ids.size() <= n && (!base || q->ids.size() > base->ids.size()) && std::equal(q->ids.begin(), q->ids.end(), ids)) base = q;
+        }
+        const int from = base ? (int)base->ids.size() : 0;
+        const int need = (n + MI_PROMPT_PAGE - 1) / MI_PROMPT_PAGE - from / MI_PROMPT_PAGE;
+        if (!h->prompt_cache) {
+            h->prompt_pages = std::max(16, need);
+            mi_prompt_cache_cfg g{};
+            g.n_layers = c.n_layers; g.n_kv_heads = c.n_kv_heads; g.head_dim = c.head_dim; g.dtype = MI_DTYPE_BF16;
+            g.n_pages = h->prompt_pages; g.max_entries = 2 * max_prompts; g.max_tokens = c.max_seq_len;   // (dropped prompts live until their passes are issued)
+            if (mi_prompt_cache_create(&g, h->device, nullptr, &h->prompt_cache)) throw Error(last_error());
+        }
+        int32_t used = 0;
+        if (mi_prompt_cache_used(h->prompt_cache, &used, nullptr)) throw Error(last_error());
+        if (used + need > h->prompt_pages) {
+            const int pages = std::max(2 * h->prompt_pages, used + need);
+            if (mi_prompt_cache_resize(h->prompt_cache, nullptr, pages, stream)) throw Error(last_error());
+            h->prompt_pages = pages;
+        }
+        auto p = std::make_shared<mi_encoder::Prompt>();
+        p->cache = h->prompt_cache;
+        p->stream = stream;
+        p->device = h->device;
+        p->ids.assign(ids, ids + n);
+        if (base ? mi_prompt_cache_fork(h->prompt_cache, base->entry, 1, &p->entry, stream) : mi_prompt_cache_new(h->prompt_cache, stream, &p->entry))
+            throw Error(last_error());
+        if (mi_prompt_cache_reserve(h->prompt_cache, p->entry, n - from, stream)) throw Error(last_error());
+        const int H = c.hidden;
+        float *sum = p->sum.as<float>((size_t)H);
+        const float *base_sum = base ? base->sum.get<float>() : nullptr;
+        const int own = n - from;
+        if (own) {
+            EncLease lease = lease_ws(h, stream);
+            mi_encoder::WS &ws = lease.w;
+            const int32_t cu[2] = {0, own};
+            Batch b = prepare_batch(h, ws, 1, ids + from, cu, nullptr, st, from);
+            b.prompted = true; b.prompt_len = from; b.store = p->entry;
+            run_stack(h, ws, b, st);
+            bf16_t *xn = ws.ws_xn.as<bf16_t>((size_t)b.T_pad * H);
+            hipLaunchKernelGGL(rmsnorm_kernel, dim3((b.T_real + 3) / 4), dim3(256), 0, st, ws.ws_x.get<float>(), h->norm_w.get<float>(), H, b.T_real,
+                               c.rms_eps, xn);
+            MI_HIP(hipGetLastError());
+            hipLaunchKernelGGL(prompt_sum_kernel, dim3((unsigned)((H + 255) / 256)), dim3(256), 0, st, xn, own, H, base_sum, sum);
+            MI_HIP(hipGetLastError());
+            MI_HIP(hipStreamSynchronize(st));              // (every stream may use the prompt from here on)
+        } else {
+            MI_HIP(hipMemcpyAsync(sum, base_sum, (size_t)H * 4, hipMemcpyDeviceToDevice, st));
+            MI_HIP(hipStreamSynchronize(st));
+        }
+        *prompt = h->next_prompt++;
+        h->prompts[*prompt] = std::move(p);
+    });
+}
+
+int mi_encoder_drop_prompt(mi_encoder *h, int32_t prompt) {
+    return guard([&] {
+        MI_REQUIRE(h, "null argument");
+        std::shared_ptr<mi_encoder::Prompt> p;               // (its end, which may wait for the device, outside the lock)
+        std::lock_guard<std::mutex> pl(h->prompts_mu);
+        auto it = h->prompts.find(prompt);
+        MI_REQUIRE(it != h->prompts.end(), "no such cached prompt");
+        p = std::move(it->second);
+        h->prompts.erase(it);
+    });
+}
+
+int mi_encoder_encode_prompted(mi_encoder *h, int32_t prompt, int nseq, const int32_t *ids, const int32_t *cu, int normalize, float *out,
+                               const int32_t *out_rows, void *stream) {
+    return guard([&] {
+        MI_REQUIRE(h, "null argument");
+        MI_REQUIRE(!out_rows || !is_device_ptr(out_rows), "mi_encoder_encode_prompted: out_rows is a host array");
+        std::shared_ptr<mi_encoder::Prompt> p;
+        {
+            std::lock_guard<std::mutex> pl(h->prompts_mu);
+            auto it = h->prompts.find(prompt);
+            MI_REQUIRE(it != h->prompts.end(), "no such cached prompt");
+            p = it->second;
+        }
+        encode_impl(h, nseq, ids, cu, normalize, out, out_rows, stream, p);
     });
 }
 
@@ -1752,6 +1921,7 @@ int mi_enc_debug_counter(const char *name, int64_t *value) {
         else if (std::string(name) == "few_ao_passes") *value = g_few_ao_passes.load();
         else if (std::string(name) == "few_gu8_passes") *value = g_few_gu8_passes.load();
         else if (std::string(name) == "few_qkv8_passes") *value = g_few_qkv8_passes.load();
+        else if (std::string(name) == "prompted_passes") *value = g_prompted_passes.load();
         else if (std::string(name) == "mid_launches") *value = g_mid_launches.load();
         else if (std::string(name) == "short_attn_launches") *value = g_short_attn_launches.load();
         else throw Error(std::string("unknown debug counter: ") + name);

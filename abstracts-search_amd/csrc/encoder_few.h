@@ -1263,6 +1263,8 @@ struct FewPoolArgs {
     const bf16_t *dense_w;         // [out_dim][H]
     const float *dense_b;          // [out_dim] or null
     float *raw;                    // [nseq][out_dim]
+    const float *prompt_sum;       // [H]: a cached prompt's share of the sums (null: none), and its length
+    int prompt_len;
 };
 
 __global__ void __launch_bounds__(256) few_pool_kernel(FewPoolArgs a) {
@@ -1294,9 +1296,13 @@ __global__ void __launch_bounds__(256) few_pool_kernel(FewPoolArgs a) {
                     }
                 }
         }
-        const float invL = 1.0f / (float)max(L, 1);
+        const float invL = 1.0f / (float)max(L + a.prompt_len, 1);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) pooled[tid * 8 + q] = bf2f(f2bf(((acc[0][q] + acc[1][q]) + (acc[2][q] + acc[3][q])) * invL));
+        for (int q = 0; q < 8; ++q) {
+            float sum = (acc[0][q] + acc[1][q]) + (acc[2][q] + acc[3][q]);
+            if (a.prompt_sum) sum += a.prompt_sum[tid * 8 + q];
+            pooled[tid * 8 + q] = bf2f(f2bf(sum * invL));
+        }
     }
     __syncthreads();
     const int per = (a.out_dim + a.parts - 1) / a.parts;

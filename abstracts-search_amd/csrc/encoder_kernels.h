@@ -2325,6 +2325,8 @@ struct PoolArgs {
     int parts;               // gridDim.y: the Dense rows are split over `parts` workgroups per sequence
                              // (few sequences: one workgroup streaming the whole Dense matrix is
                              // latency-bound, 536 us for a single query); > 1 => l2norm_rows_kernel follows
+    const float *prompt_sum; // [H]: what a cached prompt's tokens add to every sequence's sum (null: none), and how many they are
+    int prompt_len;
 };
 
 __global__ void __launch_bounds__(256) pool_kernel(PoolArgs a) {
@@ -2353,7 +2355,7 @@ __global__ void __launch_bounds__(256) pool_kernel(PoolArgs a) {
     // sequences share a pass only through the f32 summation order of the Dense dot products (~1e-7)
     // (a thread takes 4 adjacent columns: the four tokens of a step are four independent 16-byte loads -- one column per
     // thread was a chain of 4-byte strided loads, 43 us for one 31-token query)
-    const float invL = 1.0f / (float)max(L, 1);
+    const float invL = 1.0f / (float)max(L + a.prompt_len, 1);
     const int Hv = (H & 3) == 0 ? H : 0;                   // rows are 16-byte aligned only when H % 4 == 0
     for (int c = tid * 4; c < Hv; c += 1024) {
         const float4 g = *reinterpret_cast<const float4 *>(a.norm_w + c);
@@ -2378,7 +2380,11 @@ __global__ void __launch_bounds__(256) pool_kernel(PoolArgs a) {
             a4[0][2] += bf2f(f2bf(v.z * it * g.z)); a4[0][3] += bf2f(f2bf(v.w * it * g.w));
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pooled[c + k] = bf2f(f2bf(((a4[0][k] + a4[1][k]) + (a4[2][k] + a4[3][k])) * invL));
+        for (int k = 0; k < 4; ++k) {
+            float sum = (a4[0][k] + a4[1][k]) + (a4[2][k] + a4[3][k]);
+            if (a.prompt_sum) sum += a.prompt_sum[c + k];
+            pooled[c + k] = bf2f(f2bf(sum * invL));
+        }
     }
     for (int c = Hv + tid; c < H; c += 256) {               // (H % 4 != 0: one column per thread)
         const float g = a.norm_w[c];
@@ -2390,7 +2396,9 @@ __global__ void __launch_bounds__(256) pool_kernel(PoolArgs a) {
             for (int u = 0; u < 4; ++u) a4[u] += bf2f(f2bf(col[(size_t)(t + u) * H] * inv[t + u] * g));
         }
         for (; t < L; ++t) a4[0] += bf2f(f2bf(col[(size_t)t * H] * inv[t] * g));
-        pooled[c] = bf2f(f2bf(((a4[0] + a4[1]) + (a4[2] + a4[3])) * invL));
+        float sum = (a4[0] + a4[1]) + (a4[2] + a4[3]);
+        if (a.prompt_sum) sum += a.prompt_sum[c];
+        pooled[c] = bf2f(f2bf(sum * invL));
     }
     __syncthreads();
     const int parts = max(1, a.parts), part = blockIdx.y;
@@ -2441,9 +2449,10 @@ __global__ void __launch_bounds__(256) pool_kernel(PoolArgs a) {
 
 // Mean over the real tokens of every sequence of the (final-norm) bf16 rows xn [T_pad][H] -> bf16 [nseq][H]: the
 // pooling step when there are many sequences (grid: nseq x H / 512; a thread owns two columns and walks the tokens
-// with four independent accumulators per column, summed in a fixed order).
+// with four independent accumulators per column, summed in a fixed order).  prompt_sum / prompt_len: a cached prompt's share (PoolArgs).
 __global__ void __launch_bounds__(256) meanpool_kernel(const bf16_t *__restrict__ xn, const int32_t *__restrict__ seq_start,
-                                                       const int32_t *__restrict__ seq_len, int H, bf16_t *__restrict__ out) {
+                                                       const int32_t *__restrict__ seq_len, int H, bf16_t *__restrict__ out,
+                                                       const float *__restrict__ prompt_sum, int prompt_len) {
     const int seq = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 2;
     if (c >= H) return;
     const int s0 = seq_start[seq], L = seq_len[seq];
@@ -2463,9 +2472,26 @@ __global__ void __launch_bounds__(256) meanpool_kernel(const bf16_t *__restrict_
         a0[0] += __uint_as_float(v << 16);
         a1[0] += __uint_as_float(v & 0xffff0000u);
     }
-    const float inv = 1.0f / (float)max(L, 1);
-    *reinterpret_cast<unsigned *>(out + (size_t)seq * H + c) =
-        pack2(((a0[0] + a0[1]) + (a0[2] + a0[3])) * inv, ((a1[0] + a1[1]) + (a1[2] + a1[3])) * inv);
+    const float inv = 1.0f / (float)max(L + prompt_len, 1);
+    float s0_ = (a0[0] + a0[1]) + (a0[2] + a0[3]), s1_ = (a1[0] + a1[1]) + (a1[2] + a1[3]);
+    if (prompt_sum) { s0_ += prompt_sum[c]; s1_ += prompt_sum[c + 1]; }
+    *reinterpret_cast<unsigned *>(out + (size_t)seq * H + c) = pack2(s0_ * inv, s1_ * inv);
+}
+
+// out[c] = (base ? base[c] : 0) + sum over the rows of xn [T][H] (bf16): what a prompt's tokens add to the pooling, four accumulators
+// a column in f32, once per prompt
+__global__ void __launch_bounds__(256) prompt_sum_kernel(const bf16_t *__restrict__ xn, int T, int H, const float *__restrict__ base,
+                                                         float *__restrict__ out) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= H) return;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    int t = 0;
+    for (; t + 4 <= T; t += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[u] += bf2f(xn[(size_t)(t + u) * H + c]);
+    for (; t < T; ++t) a[0] += bf2f(xn[(size_t)t * H + c]);
+    const float sum = (a[0] + a[1]) + (a[2] + a[3]);
+    out[c] = base ? base[c] + sum : sum;
 }
 
 // L2 normalisation of the rows of out[nseq][n] (second step of a split pool_kernel)

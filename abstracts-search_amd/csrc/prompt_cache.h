@@ -7,11 +7,12 @@
 
 namespace mi {
 
-// the encoder's own operand forms (PromptArgs: vt, inter, frag)
+// the encoder's own operand forms (PromptArgs: vt, inter, frag), and an entry that is being filled
 struct PromptForms {
     bool vt = false, inter = false;
     void *frag = nullptr;
     int frag_mt = 0;
+    int prompt_tokens = -1;      // attend to this many of the entry's tokens (-1: all)
 };
 int64_t prompt_attention_workspace(mi_prompt_cache *c, const mi_prompt_attn &a);
 void prompt_attention(mi_prompt_cache *c, const mi_prompt_attn &a, const PromptForms &f, void *stream);

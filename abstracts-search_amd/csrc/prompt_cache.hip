@@ -184,7 +184,7 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     a.out = static_cast<bf16_t *>(x.out);
     a.q_token = x.q_token; a.q_head = x.q_head; a.k_token = x.k_token; a.k_head = x.k_head; a.v_token = x.v_token; a.v_head = x.v_head;
     a.o_token = x.o_token; a.o_head = x.o_head;
-    a.pages = c->pages + x.layer * c->layer_stride; a.page_stride = c->page_stride; a.table = c->table(x.entry); a.P = e.len;
+    a.pages = c->pages + x.layer * c->layer_stride; a.page_stride = c->page_stride; a.table = c->table(x.entry); a.P = f.prompt_tokens < 0 ? e.len : std::min(f.prompt_tokens, e.len);
     a.n_tokens = x.n_tokens; a.n_keys = x.n_keys; a.n_texts = x.n_texts; a.cu_q = x.cu_q; a.cu_k = x.cu_k;
     a.n_heads = x.n_heads; a.n_kv = g.n_kv_heads; a.G = x.n_heads / g.n_kv_heads; a.causal = x.causal; a.zero_rest = x.zero_rest;
     a.scale2 = std::max(x.scale * 1.4426950408889634f, 1e-30f);   // (0 means equal weights; a masked score is -inf, and 0 x inf is no number)

@@ -56,6 +56,9 @@ class _Lib:
                 "mi_encoder_out_dim": [v, POINTER(c_int)],
                 "mi_encoder_encode": [v, c_int, v, v, c_int, v, v],
                 "mi_encoder_encode_rows": [v, c_int, v, v, c_int, v, v, v],
+                "mi_encoder_cache_prompt": [v, c_int, v, POINTER(c_int32), v],
+                "mi_encoder_drop_prompt": [v, c_int32],
+                "mi_encoder_encode_prompted": [v, c_int32, c_int, v, v, c_int, v, v, v],
                 "mi_encoder_hidden": [v, c_int, v, v, v, v],
                 "mi_encoder_profile_enable": [v, c_int],
                 "mi_encoder_profile_read": [v, POINTER(c_double), POINTER(c_double)],
@@ -239,6 +242,7 @@ class SentenceTransformer:
         if causal is not None:
             cfg["causal"] = bool(causal)
         self.config = cfg
+        self._cached_prompts: dict = {}          # token ids of a cached prompt -> its handle
         c = _Cfg(**{k: (int(v) if isinstance(v, bool) else v) for k, v in cfg.items() if k in dict(_Cfg._fields_)})
         self._h = c_void_p()
         _check(_Lib.get().mi_encoder_create(ctypes.byref(c), self._device_index, ctypes.byref(self._h)))
@@ -323,6 +327,7 @@ class SentenceTransformer:
         """name -> torch tensor / numpy array (f32, bf16 or f16; host or CUDA)."""
         import torch
         lib = _Lib.get()
+        self._cached_prompts = {}                # (a new weight makes the library drop them)
         for name, t in weights.items():
             if name.startswith("model."):
                 name = name[6:]
@@ -387,6 +392,59 @@ class SentenceTransformer:
             emb = emb[0]
         return emb
 
+    # -- prompts computed once ------------------------------------------
+    def _prompt_tokens(self, prompt: str):
+        """the token ids that every text behind `prompt` begins with: what its tokenisations with different continuations have
+        in common (a tokenizer may join the prompt's last characters with the text's first ones, and end the ids with its own
+        special tokens)"""
+        tries = self.tokenize([prompt + s for s in ("a", "The", "0", "(", " x")])
+        n = 0
+        while all(n < len(t) for t in tries) and len({t[n] for t in tries}) == 1:
+            n += 1
+        return list(tries[0][:n])
+
+    def cache_prompt(self, prompt=None, prompt_name: str | None = None) -> int:
+        """Computes a prompt once: `encode` and `encode_tokens` then run only the texts' own tokens behind it.
+
+        `prompt`: the string that `encode(prompt=...)` puts in front of every text, or a list of token ids; `prompt_name`: one of
+        `prompts` (None: the default prompt).  Causal models only -- in a bidirectional one (stella, gte-Qwen2) the prompt's
+        hidden states depend on the text behind it.  Returns how many tokens are held; the embeddings are the same to bf16
+        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before.  A prompt that begins as one
+        that is cached shares its pages.  `load_weights` drops all of them."""
+        import torch
+        if not self.config.get("causal"):
+            raise ValueError("cache_prompt needs a causal model: in a bidirectional one the prompt's hidden states depend on the text behind it")
+        if prompt is None:
+            name = prompt_name or self.default_prompt_name
+            if name not in self.prompts:
+                raise ValueError(f"Prompt name '{name}' not found in the configured prompts dictionary with keys {list(self.prompts)!r}.")
+            prompt = self.prompts[name]
+        ids = self._prompt_tokens(prompt) if isinstance(prompt, str) else [int(i) for i in prompt]
+        if not ids or len(ids) >= self.max_seq_length:
+            raise ValueError(f"cache_prompt: a prompt of 1 .. {self.max_seq_length - 1} tokens, got {len(ids)}")
+        key = tuple(ids)
+        if key not in self._cached_prompts:
+            a, n = np.asarray(ids, np.int32), c_int32()
+            stream = c_void_p(torch.cuda.current_stream(torch.device("cuda", self._device_index)).cuda_stream)
+            _check(_Lib.get().mi_encoder_cache_prompt(self._h, len(ids), c_void_p(a.ctypes.data), ctypes.byref(n), stream))
+            self._cached_prompts[key] = n.value
+        return len(ids)
+
+    def drop_prompts(self) -> None:
+        """forgets every cached prompt"""
+        cached, self._cached_prompts = self._cached_prompts, {}
+        for handle in cached.values():
+            _check(_Lib.get().mi_encoder_drop_prompt(self._h, handle))
+
+    def _behind(self, ids):
+        """(length, handle) of the longest cached prompt that `ids` goes on from, else (0, None)"""
+        best = (0, None)
+        for key, handle in self._cached_prompts.items():
+            n = len(key)
+            if best[0] < n < len(ids) and tuple(ids[:n]) == key:
+                best = (n, handle)
+        return best
+
     # Tokens one forward pass takes: 32 768 = 128 row tiles of 256, with which every GEMM of the stack fills whole
     # rounds of the 256 CUs (N = 1536: 768 tiles = 3.0 rounds, 2048: 4.0, 17 920: 35.0).  sentence-transformers'
     # batch_size (32 by default) is a memory knob of its hardware; the token budget is the memory bound here
@@ -420,14 +478,29 @@ class SentenceTransformer:
         inputs are sorted by length (longest first) before batching and the
         result is put back in input order; a batch is packed, not padded, and holds at most
         `token_budget` tokens (see above) and at most `batch_size` sequences (None: no bound)."""
-        import itertools
         import torch
         n = len(token_lists)
         dim = self.get_sentence_embedding_dimension()
         dev = torch.device("cuda", self._device_index)
         out = torch.empty((n, dim), dtype=torch.float32, device=dev)
-        order = sorted(range(n), key=lambda i: -len(token_lists[i]))
         stream = c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        groups = [(None, list(range(n)))]
+        if self._cached_prompts:                 # texts behind the same cached prompt share passes, without its tokens
+            by: dict = {}
+            behind = [self._behind(t) for t in token_lists]
+            for i, (_, handle) in enumerate(behind):
+                by.setdefault(handle, []).append(i)
+            token_lists = [t[k:] for t, (k, _) in zip(token_lists, behind)]
+            groups = list(by.items())
+        for handle, members in groups:
+            order = sorted(members, key=lambda i: -len(token_lists[i]))
+            self._encode_group(handle, order, token_lists, batch_size, normalize_embeddings, out, stream)
+        if as_tensor:
+            return out
+        return out.cpu().numpy()
+
+    def _encode_group(self, handle, order, token_lists, batch_size, normalize_embeddings, out, stream):
+        import itertools
         lib = _Lib.get()
         # every pass only ENQUEUES work (the C ABI stages the token ids through pinned memory and writes embedding i
         # straight to row sel[i] of `out`): the packing of the next pass overlaps the GPU running this one
@@ -439,12 +512,9 @@ class SentenceTransformer:
             else:
                 ids = np.fromiter(itertools.chain.from_iterable(token_lists[i] for i in sel), np.int32, count=int(cu[-1]))
             rows = np.asarray(sel, np.int32)
-            _check(lib.mi_encoder_encode_rows(self._h, len(sel), c_void_p(ids.ctypes.data), c_void_p(cu.ctypes.data),
-                                              int(normalize_embeddings), c_void_p(out.data_ptr()), c_void_p(rows.ctypes.data),
-                                              stream))
-        if as_tensor:
-            return out
-        return out.cpu().numpy()
+            args = (len(sel), c_void_p(ids.ctypes.data), c_void_p(cu.ctypes.data), int(normalize_embeddings), c_void_p(out.data_ptr()),
+                    c_void_p(rows.ctypes.data), stream)
+            _check(lib.mi_encoder_encode_rows(self._h, *args) if handle is None else lib.mi_encoder_encode_prompted(self._h, handle, *args))
 
     # -- parity / measurement hooks ---------------------------------------
     def last_hidden_state(self, token_lists):

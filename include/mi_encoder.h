@@ -81,6 +81,19 @@ int mi_encoder_encode(mi_encoder *h, int nseq, const int32_t *ids, const int32_t
 int mi_encoder_encode_rows(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu_seqlens,
                            int normalize, float *out, const int32_t *out_rows, void *stream);
 
+/* Prompts computed once (causal models: cfg.causal).  Texts are encoded behind an instruction prompt (reference README.md:28,
+ * PROMPT_NAME); in a causal model the prompt's keys, values and hidden states do not depend on the text behind it.
+ * mi_encoder_cache_prompt runs the n tokens of a prompt once and keeps their keys and values (in pages of the prompt cache
+ * below: a prompt that begins as a cached one shares its full pages and runs only the tokens behind it) and what they add to
+ * the mean pooling; it returns when the prompt is ready, on any stream.  mi_encoder_encode_prompted encodes texts behind it --
+ * `ids` hold each text's own tokens alone, at least one, prompt and text together at most max_seq_len -- and gives what
+ * mi_encoder_encode gives for prompt + text, to bf16 rounding.  out_rows as for mi_encoder_encode_rows, or NULL.  Loading a
+ * weight drops all cached prompts. */
+int mi_encoder_cache_prompt(mi_encoder *h, int n, const int32_t *ids, int32_t *prompt, void *stream);
+int mi_encoder_drop_prompt(mi_encoder *h, int32_t prompt);
+int mi_encoder_encode_prompted(mi_encoder *h, int32_t prompt, int nseq, const int32_t *ids, const int32_t *cu_seqlens,
+                               int normalize, float *out, const int32_t *out_rows, void *stream);
+
 /* Parity hook: the stack's last hidden state after the final norm,
  * float32 [T][hidden] (host or device), packed like ids. */
 int mi_encoder_hidden(mi_encoder *h, int nseq, const int32_t *ids, const int32_t *cu_seqlens,
@@ -97,7 +110,7 @@ int mi_encoder_profile_read(mi_encoder *h, double *gemm_ms, double *gemm_flops);
  * launches whose last (partial) round of 256x256 tiles was split along K with f32 atomics into the residual stream;
  * "splitk_launches" = residual GEMMs whose every tile was split along K through the workspace (a few hundred to ~5 000
  * tokens); "reduce_norm_launches" = those whose reduction pass also wrote the next RMSNorm; "n192_launches" = residual
- * GEMMs run on 256 x 192 tiles. */
+ * GEMMs run on 256 x 192 tiles; "prompted_passes" = forward passes behind a cached prompt (and those that cached one). */
 int mi_enc_debug_counter(const char *name, int64_t *value);
 
 /* The library reads its MI_* environment knobs (README.md lists them; each overrides a measured dispatch rule) ONCE, at the

@@ -1,0 +1,206 @@
+"""GPU tests of encoding behind a cached prompt (SentenceTransformer.cache_prompt -> mi_encoder_encode_prompted): the embeddings
+of prompt + text against the fp32 oracle (cosine within 1e-3, the encoder's bound) and against the uncached path, through every
+regime of token counts the encoder has."""
+from dataclasses import replace
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def st():
+    import abstracts_search_amd.sentence_transformers as m
+    return m
+
+
+@pytest.fixture(scope="module")
+def tiny():
+    from oracle import encoder_oracle as E
+    cfg = replace(E.TINY, causal=True, max_seq_len=400)
+    return cfg, E.synth_weights(cfg, 11)
+
+
+def oracle_encode(cfg, W, toks):
+    from oracle import encoder_oracle as E
+    cu = np.concatenate([[0], np.cumsum([len(t) for t in toks])])
+    return E.encode(cfg, W, np.concatenate(toks), cu, True).numpy()
+
+
+def same(a, b, cos):
+    assert np.isfinite(a).all() and np.isfinite(b).all()
+    c = (a * b).sum(1) / np.maximum(np.linalg.norm(a, axis=1) * np.linalg.norm(b, axis=1), 1e-30)
+    assert c.min() > 1 - cos, c.min()
+
+
+@pytest.mark.parametrize("prompt_len", [1, 7, 63, 64, 65, 200])
+@pytest.mark.parametrize("lens", [[1], [9], [30], [17, 1, 20], [1] * 40, [60, 3, 90], [120, 77, 150, 31]])
+def test_prompted_against_the_oracle(st, tiny, prompt_len, lens):
+    cfg, W = tiny
+    rng = np.random.default_rng(prompt_len * 100 + len(lens))
+    prompt = rng.integers(0, cfg.vocab_size, prompt_len).tolist()
+    toks = [prompt + rng.integers(0, cfg.vocab_size, n).tolist() for n in lens]
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    plain = model.encode_tokens(toks, normalize_embeddings=True)
+    raw = model.encode_tokens(toks)
+    p0 = st.debug_counter("prompted_passes")
+    assert model.cache_prompt(prompt) == prompt_len
+    e = model.encode_tokens(toks, normalize_embeddings=True)
+    assert st.debug_counter("prompted_passes") == p0 + 2         # the prompt's own pass and one for the texts
+    ref = oracle_encode(cfg, W, toks)
+    same(e, ref, 1e-3)
+    same(e, plain, 1e-3)
+    same(model.encode_tokens(toks), raw, 1e-3)
+    assert np.allclose(np.linalg.norm(model.encode_tokens(toks), axis=1), np.linalg.norm(raw, axis=1), rtol=2e-2)
+    assert np.array_equal(e, model.encode_tokens(toks, normalize_embeddings=True))     # the same bits every time
+    model.drop_prompts()
+    p1 = st.debug_counter("prompted_passes")
+    assert np.array_equal(plain, model.encode_tokens(toks, normalize_embeddings=True))
+    assert st.debug_counter("prompted_passes") == p1
+
+
+@pytest.mark.parametrize("knob", [None, "MI_NO_FEW", "MI_NO_FEW_QKV8", "MI_NO_ROPE_FUSE"])
+def test_prompted_at_the_real_width(st, knob, monkeypatch):
+    """two layers of stella's width, causal: the query-time path, the few-hundred-token tiles and the many-token slab GEMMs (whose
+    Q and K leave with their rotary pairs interleaved), one prompt computed by one of them and read by all"""
+    if knob:
+        monkeypatch.setenv(knob, "1")
+    cfg = dict(st.STELLA_EN_1_5B_V5, vocab_size=2048, n_layers=2, causal=True, max_seq_len=700)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    H, I, hd = cfg["hidden"], cfg["intermediate"], cfg["head_dim"]
+    qc, kc = cfg["n_heads"] * hd, cfg["n_kv_heads"] * hd
+    rnd = lambda shape, scale: (torch.randn(shape, generator=g, device="cuda") * scale).bfloat16()
+    W = {"embed_tokens.weight": rnd((2048, H), 0.3), "norm.weight": torch.ones(H, device="cuda"), "dense.weight": rnd((1024, H), H ** -0.5),
+         "dense.bias": torch.zeros(1024, device="cuda")}
+    for l in range(2):
+        p = f"layers.{l}."
+        W.update({p + "input_layernorm.weight": torch.ones(H, device="cuda"), p + "post_attention_layernorm.weight": torch.ones(H, device="cuda"),
+                  p + "self_attn.q_proj.weight": rnd((qc, H), H ** -0.5), p + "self_attn.q_proj.bias": rnd((qc,), 0.3),
+                  p + "self_attn.k_proj.weight": rnd((kc, H), H ** -0.5), p + "self_attn.k_proj.bias": rnd((kc,), 0.3),
+                  p + "self_attn.v_proj.weight": rnd((kc, H), H ** -0.5), p + "self_attn.v_proj.bias": rnd((kc,), 0.1),
+                  p + "self_attn.o_proj.weight": rnd((H, qc), qc ** -0.5), p + "mlp.gate_proj.weight": rnd((I, H), H ** -0.5),
+                  p + "mlp.up_proj.weight": rnd((I, H), H ** -0.5), p + "mlp.down_proj.weight": rnd((H, I), I ** -0.5)})
+    model = st.SentenceTransformer(config=cfg, weights=W)
+    rng = np.random.default_rng(6)
+    for prompt_len in (20, 130, 333):                             # computed by the query-time path, by the mid and by the slab tiles
+        prompt = rng.integers(0, 2048, prompt_len).tolist()
+        batches = [[rng.integers(0, 2048, int(n)).tolist() for n in lens] for lens in
+                   ([12], [40], [8, 20, 9], rng.integers(5, 60, 12), rng.integers(30, 300, 60))]
+        plain = [model.encode_tokens([prompt + t for t in b], normalize_embeddings=True) for b in batches]
+        model.cache_prompt(prompt)
+        for b, want in zip(batches, plain):
+            same(model.encode_tokens([prompt + t for t in b], normalize_embeddings=True), want, 2e-4)
+        model.drop_prompts()
+
+
+def test_prompts_that_begin_alike_and_texts_without_one(st, tiny):
+    """prompts that extend each other (shared pages), texts behind each, behind none, and one that is a cached prompt itself"""
+    cfg, W = tiny
+    rng = np.random.default_rng(3)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    a = rng.integers(0, cfg.vocab_size, 100).tolist()
+    b, c = a + rng.integers(0, cfg.vocab_size, 70).tolist(), a + rng.integers(0, cfg.vocab_size, 28).tolist()
+    other = rng.integers(0, cfg.vocab_size, 30).tolist()
+    text = lambda n: rng.integers(0, cfg.vocab_size, n).tolist()
+    toks = [b + text(10), other + text(4), a + text(50), c + text(3), a, b, other, c + text(150), [5], b + text(1), a[:40]]
+    ref = oracle_encode(cfg, W, toks)
+    for order in ([a, b, c, other], [b, other, a, c], [c, b, a]):
+        for p in order:
+            model.cache_prompt(p)
+        model.cache_prompt(order[0])                              # again: nothing to do
+        for bs in (None, 2):
+            same(model.encode_tokens(toks, normalize_embeddings=True, batch_size=bs), ref, 1e-3)
+        model.drop_prompts()
+    # many prompts: the pool grows, and what is cached stays right
+    grown = [a + text(60 + i) for i in range(30)]
+    for p in grown:
+        model.cache_prompt(p)
+    toks = [p + text(5) for p in grown]
+    same(model.encode_tokens(toks, normalize_embeddings=True), oracle_encode(cfg, W, toks), 1e-3)
+
+
+def test_prompted_on_other_streams_and_threads(st, tiny):
+    import threading
+    cfg, W = tiny
+    rng = np.random.default_rng(8)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    prompt = rng.integers(0, cfg.vocab_size, 150).tolist()
+    work = [[prompt + rng.integers(0, cfg.vocab_size, int(n)).tolist() for n in rng.integers(1, 90, 6)] for _ in range(4)]
+    model.cache_prompt(prompt)
+    want = [model.encode_tokens(w, normalize_embeddings=True) for w in work]
+    got, errors = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = model.encode_tokens(work[i], normalize_embeddings=True)
+        except Exception as e:                                    # pragma: no cover
+            errors.append(e)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    for k in range(6):                                            # prompts come meanwhile, and the pool grows
+        model_ids = rng.integers(0, cfg.vocab_size, 350).tolist()
+        n = st.c_int32()
+        a = np.asarray(model_ids, np.int32)
+        st._check(st._Lib.get().mi_encoder_cache_prompt(model._h, len(a), a.ctypes.data, st.ctypes.byref(n), None))
+        if k % 2:
+            st._check(st._Lib.get().mi_encoder_drop_prompt(model._h, n.value))
+    [t.join() for t in ts]
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w)
+
+
+def test_encode_with_a_prompt_string(st, tiny):
+    """encode(prompt_name=..) on a model with a tokenizer: the cached prompt is found behind the string, also where the tokenizer
+    appends its own token to every text"""
+    from tokenizers import Tokenizer, models, pre_tokenizers
+    cfg, W = tiny
+    words = ["[UNK]", "Instruct", ":", "find", "papers", "Query", "a", "0", "The", "(", "x"] + [f"w{i}" for i in range(40)] + ["</s>"]
+    tk = Tokenizer(models.WordLevel({w: i for i, w in enumerate(words)}, unk_token="[UNK]"))
+    tk.pre_tokenizer = pre_tokenizers.Whitespace()
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W, tokenizer=tk, prompts={"q": "Instruct: find papers\nQuery: "})
+    model._host_tok.eos_id = words.index("</s>")
+    texts = ["w1 w2", "w3", "w9 w9 w9 w30 a"]
+    plain = model.encode(texts, prompt_name="q", normalize_embeddings=True)
+    assert model.cache_prompt(prompt_name="q") == 6
+    p0 = st.debug_counter("prompted_passes")
+    same(model.encode(texts, prompt_name="q", normalize_embeddings=True), plain, 1e-3)
+    assert st.debug_counter("prompted_passes") == p0 + 1
+    one = model.encode("w1 w2", prompt_name="q", normalize_embeddings=True)
+    same(one[None], plain[:1], 1e-3)
+    same(model.encode(texts, normalize_embeddings=True), oracle_encode(cfg, W, model.tokenize(texts)), 1e-3)
+
+
+def test_refusals(st, tiny):
+    cfg, W = tiny
+    two = replace(cfg, causal=False)
+    both = st.SentenceTransformer(config=two.to_dict(), weights=W)
+    with pytest.raises(ValueError, match="causal"):
+        both.cache_prompt([1, 2, 3])
+    lib, n, a = st._Lib.get(), st.c_int32(), np.asarray([1, 2, 3], np.int32)
+    assert lib.mi_encoder_cache_prompt(both._h, 3, a.ctypes.data, st.ctypes.byref(n), None) != 0 and b"causal" in lib.mi_enc_last_error()
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    for bad in ([], [1] * 400):
+        with pytest.raises(ValueError):
+            model.cache_prompt(bad)
+    with pytest.raises(RuntimeError, match="out of range"):
+        model.cache_prompt([1, cfg.vocab_size])
+    with pytest.raises(ValueError, match="not found"):
+        model.cache_prompt(prompt_name="nope")
+    model.cache_prompt([1] * 390)
+    h = next(iter(model._cached_prompts.values()))
+    out, ids = torch.empty(1, 64, device="cuda"), np.ones(11, np.int32)
+    run = lambda handle, ids: lib.mi_encoder_encode_prompted(model._h, handle, 1, ids.ctypes.data, np.asarray([0, len(ids)], np.int32).ctypes.data, 1,
+                                                              out.data_ptr(), None, None)
+    assert run(h, ids) != 0 and b"longer than max_seq_len" in lib.mi_enc_last_error()
+    assert run(h + 1, ids[:3]) != 0 and b"no such cached prompt" in lib.mi_enc_last_error()
+    assert run(h, ids[:10]) == 0
+    assert lib.mi_encoder_drop_prompt(model._h, h + 1) != 0
+    model.load_weights({"norm.weight": W["norm.weight"]})         # (drops the prompts)
+    assert run(h, ids[:3]) != 0 and not model._cached_prompts
+    torch.cuda.synchronize()
