@@ -473,6 +473,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
         f32x16 s[2];
         const bool own = i >= np;
         const int b = base_of(i), l = own ? lo - b : 0, h = (own ? hi : a.P) - b;   // the row sees keys [l, h) of the chunk
+        const unsigned from = (unsigned)(8 * half) - (unsigned)l, span = (unsigned)max(h - l, 0);
         auto read_k = [&](int f) { kf[f & 3] = lds_16(Ks + (krow + 32 * (f / NKK)) * HD + (((2 * (f % NKK) + half) ^ kkey) * 8)); };
         auto read_v = [&](int g) {
             const int J = g / NDT, n = g % NDT;
@@ -489,9 +490,9 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
             constexpr int j = decltype(J_)::value;
             if (md == MASK) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = 32 * j + 16 * (r >> 3) + 8 * half + (r & 7);
-                    if (key < l || key >= h) s[j][r] = -__builtin_huge_valf();
+                for (int r = 0; r < 16; ++r) {                                   // (key - l as an unsigned number: one comparison for both ends)
+                    const unsigned key = (unsigned)(32 * j + 16 * (r >> 3) + (r & 7)) + from;
+                    s[j][r] = key < span ? s[j][r] : -__builtin_huge_valf();
                 }
             }
             float mx = s[j][0];

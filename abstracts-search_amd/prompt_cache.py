@@ -114,10 +114,12 @@ class PromptCache:
         _check(lib.mi_prompt_cache_create(ctypes.byref(cfg), self.device.index, self.pages.data_ptr(), ctypes.byref(self._h)))
         self._close = weakref.finalize(self, _destroy, self._h)
         self._lib = lib
-        self._current_stream = torch.cuda.current_stream
-
-    def _stream(self):
-        return self._current_stream(self.device).cuda_stream
+        self._table_cap = -(-max_tokens // PAGE) if max_tokens else n_pages   # pages of the longest entry
+        self._plans: dict = {}                       # (entry, shapes) -> bytes of workspace, until an entry changes
+        # torch's current stream as a pointer (building the Stream object first is 1.7 us of a 10 us call)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        index, device = self.device.index, self.device
+        self._stream = (lambda: raw(index)) if raw else (lambda: torch.cuda.current_stream(device).cuda_stream)
 
     # -- prompts ------------------------------------------------------------
     def new(self) -> int:
@@ -128,6 +130,7 @@ class PromptCache:
 
     def reserve(self, entry: int, n: int) -> None:
         """n more tokens at the end of the entry, to be filled by ``write``"""
+        self._plans.clear()
         _check(self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream()))
 
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
@@ -180,6 +183,7 @@ class PromptCache:
     def free(self, entries) -> None:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
+        self._plans.clear()
         _check(self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream()))
 
     def compact(self) -> int:
@@ -206,10 +210,10 @@ class PromptCache:
 
     def table(self, entry: int) -> list[int]:
         """the page numbers of the entry, in order"""
-        cap = -(-self.length(entry) // PAGE)
+        cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
-        _check(self._lib.mi_prompt_cache_entry(self._h, entry, None, t, cap))
-        return list(t)
+        _check(self._lib.mi_prompt_cache_entry(self._h, entry, ctypes.byref(n), t, cap))
+        return t[:-(-n.value // PAGE)]
 
     @property
     def n_pages(self) -> int:
@@ -234,19 +238,21 @@ class PromptCache:
         None.  out: written in place if given (tokens behind the last text keep what they hold; in a new output they are
         zeros).  Inference only: no gradient."""
         import torch
-        if q.dim() != 3 or q.shape[2] != self.head_dim:
-            raise ValueError(f"PromptCache.attention: q [tokens, heads, {self.head_dim}], got {tuple(q.shape)}")
+        hd, kv, dtype, device = self.head_dim, self.n_kv_heads, self.dtype, self.device
+        if q.dim() != 3 or q.shape[2] != hd:
+            raise ValueError(f"PromptCache.attention: q [tokens, heads, {hd}], got {tuple(q.shape)}")
         if (k is None) != (v is None):
             raise ValueError("PromptCache.attention: k and v come together")
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))):
             raise ValueError("PromptCache.attention has no gradient: call it under torch.no_grad()")
-        q = self._fit(q, "q")
+        if q.dtype != dtype or q.device != device or not q.is_contiguous() or q.data_ptr() & 15:
+            q = self._fit(q, "q")
         tokens, heads, _ = q.shape
         if k is None:
             keys, kp, vp, ks, vs = 0, 0, 0, (0, 0), (0, 0)
         else:
-            if k.dim() != 3 or k.shape != v.shape or k.shape[1] != self.n_kv_heads or k.shape[2] != self.head_dim:
-                raise ValueError(f"PromptCache.attention: k and v [keys, {self.n_kv_heads}, {self.head_dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
+            if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kv or k.shape[2] != hd:
+                raise ValueError(f"PromptCache.attention: k and v [keys, {kv}, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
             k, v = self._fit(k, "k"), self._fit(v, "v")
             keys, kp, vp, ks, vs = k.shape[0], k.data_ptr(), v.data_ptr(), k.stride(), v.stride()
         if cu_q is None:
@@ -259,25 +265,33 @@ class PromptCache:
                     raise ValueError(f"PromptCache.attention: {keys} keys for {tokens} tokens need cu_k")
                 cu_k = cu_q
             for cu in (cu_q, cu_k):
-                if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape != cu_q.shape or cu.device != self.device or not cu.is_contiguous():
-                    raise ValueError(f"PromptCache.attention: cu_q and cu_k are contiguous int32 [texts + 1] on {self.device}")
+                if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape != cu_q.shape or cu.device != device or not cu.is_contiguous():
+                    raise ValueError(f"PromptCache.attention: cu_q and cu_k are contiguous int32 [texts + 1] on {device}")
             texts, cq, ck = cu_q.shape[0] - 1, cu_q.data_ptr(), cu_k.data_ptr()
             if texts < 1:
                 raise ValueError("PromptCache.attention: no text")
         rest = out is None
         if rest:
-            out = torch.empty((tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
-        elif (out.dtype != self.dtype or out.device != self.device or out.shape != q.shape or out.stride(2) != 1 or out.data_ptr() & 15
+            out = q.new_empty((tokens, heads, hd))
+        elif (out.dtype != dtype or out.device != device or out.shape != q.shape or out.stride(2) != 1 or out.data_ptr() & 15
               or out.stride(0) & 7 or out.stride(1) & 7):
-            raise ValueError(f"PromptCache.attention: out {tuple(q.shape)} {self.dtype} on {self.device} with 16-byte aligned rows")
+            raise ValueError(f"PromptCache.attention: out {tuple(q.shape)} {dtype} on {device} with 16-byte aligned rows")
         if scale is None:
-            scale = 1.0 / math.sqrt(self.head_dim)
+            scale = hd ** -0.5
         elif not 0 <= scale < math.inf:
             raise ValueError(f"PromptCache.attention: scale must be finite and not negative, got {scale}")
-        head = (entry, layer, heads, tokens, keys, texts, q.data_ptr(), kp, vp, out.data_ptr(), q.stride(0), q.stride(1), ks[0], ks[1],
-                vs[0], vs[1], out.stride(0), out.stride(1), cq, ck, causal, scale, rest, 0)
-        need = c_int64()
-        _check(self._lib.mi_prompt_attention_workspace(self._h, _ATTN.pack(*head, 0, 0), ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        _check(self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need.value else 0, need.value), self._stream()))
+        qs, os = q.stride(), out.stride()
+        head = (entry, layer, heads, tokens, keys, texts, q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                cq, ck, causal, scale, rest, 0)
+        shape = (entry, heads, tokens, keys, texts)
+        need = self._plans.get(shape)
+        if need is None:
+            n = c_int64()
+            _check(self._lib.mi_prompt_attention_workspace(self._h, _ATTN.pack(*head, 0, 0), ctypes.byref(n)))
+            need = n.value
+            if len(self._plans) > 1000:
+                self._plans.clear()
+            self._plans[shape] = need
+        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        _check(self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need else 0, need), self._stream()))
         return out
