@@ -1765,7 +1765,7 @@ int mi_encoder_cache_prompt(mi_encoder *h, int n, const int32_t *ids, int32_t *p
         p->stream = stream;
         p->device = h->device;
         p->ids.assign(ids, ids + n);
-        if (base ? mi_prompt_cache_fork(h->prompt_cache, base->entry, 1, &p->entry, stream) : mi_prompt_cache_new(h->prompt_cache, stream, &p->entry))
+        if (base ? mi_prompt_cache_fork(h->prompt_cache, base->entry, 1, &p->entry, nullptr, stream) : mi_prompt_cache_new(h->prompt_cache, stream, &p->entry))
             throw Error(last_error());
         if (mi_prompt_cache_reserve(h->prompt_cache, p->entry, n - from, stream)) throw Error(last_error());
         const int H = c.hidden;

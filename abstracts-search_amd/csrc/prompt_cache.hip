@@ -6,7 +6,6 @@
 #include <cstring>
 #include <memory>
 #include <mutex>
-#include <set>
 #include <vector>
 
 #include "prompt_kernels.h"
@@ -25,6 +24,25 @@ bool capturing(void *stream) {
     MI_HIP(hipStreamIsCapturing(as_stream(stream), &st));
     return st != hipStreamCaptureStatusNone;
 }
+
+// a set of page numbers, read lowest first
+struct PageSet {
+    std::vector<uint64_t> bits;
+    int count = 0;
+    void reset(int n, int from) {                 // from .. n - 1
+        bits.assign(((size_t)n + 63) / 64, 0);
+        count = 0;
+        for (int p = from; p < n; ++p) insert(p);
+    }
+    void insert(int p) { bits[p >> 6] |= 1ull << (p & 63); ++count; }
+    void erase(int p) { bits[p >> 6] &= ~(1ull << (p & 63)); --count; }
+    template <class F>
+    void each(F &&f) const {                      // f(p) returns whether to go on
+        for (size_t w = 0; w < bits.size(); ++w)
+            for (uint64_t b = bits[w]; b; b &= b - 1)
+                if (!f((int32_t)(w * 64 + __builtin_ctzll(b)))) return;
+    }
+};
 
 struct Entry {
     bool live = false;
@@ -47,7 +65,7 @@ struct mi_prompt_cache {
     std::mutex mu;
     std::vector<int32_t> ref;            // entries that hold the page
     std::vector<void *> tag;             // of a free page: the stream whose work may still read it
-    std::set<int32_t> free_pages;
+    PageSet free_pages;
     std::vector<Entry> entries;
 
     Entry &at(int32_t e) {
@@ -58,15 +76,16 @@ struct mi_prompt_cache {
 
     void wait_all() {                    // everything issued so far is done: whatever is free is free for every stream
         MI_HIP(hipDeviceSynchronize());
-        for (int32_t p : free_pages) tag[p] = ANY;
+        free_pages.each([&](int32_t p) { tag[p] = ANY; return true; });
         for (Entry &e : entries)
             if (!e.live) e.slot_tag = ANY;
     }
     // the n lowest free pages, fit for use on `stream` (still free: the caller takes them once its launches are out)
     std::vector<int32_t> pick_pages(int n, void *stream) {
-        MI_REQUIRE((size_t)n <= free_pages.size(),
-                   "prompt cache: " + std::to_string(n) + " pages needed, " + std::to_string(free_pages.size()) + " free");
-        std::vector<int32_t> got(free_pages.begin(), std::next(free_pages.begin(), n));
+        if (n > free_pages.count) throw Error("prompt cache: " + std::to_string(n) + " pages needed, " + std::to_string(free_pages.count) + " free");
+        std::vector<int32_t> got;
+        got.reserve(n);
+        if (n) free_pages.each([&](int32_t p) { got.push_back(p); return (int)got.size() < n; });
         for (int32_t p : got)
             if (tag[p] != ANY && tag[p] != stream) { wait_all(); break; }
         return got;
@@ -76,7 +95,7 @@ struct mi_prompt_cache {
         std::vector<int32_t> got;
         for (int32_t e = 0; e < (int32_t)entries.size() && (int)got.size() < n; ++e)
             if (!entries[e].live) got.push_back(e);
-        MI_REQUIRE((int)got.size() == n, "prompt cache: more than max_entries (" + std::to_string(cfg.max_entries) + ") entries");
+        if ((int)got.size() != n) throw Error("prompt cache: more than max_entries (" + std::to_string(cfg.max_entries) + ") entries");
         for (int32_t e : got)
             if (entries[e].slot_tag != ANY && entries[e].slot_tag != stream) { wait_all(); break; }
         return got;
@@ -88,19 +107,46 @@ struct mi_prompt_cache {
     void reads(Entry &e, void *stream, bool cap) {
         if (cap || stream != e.home) e.foreign = true;
     }
-    void copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st);
+    // src[j] -> dst[j]; into: the new entry that the pages dst make up; kids, parent: the new entries that fork `parent`
+    void copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st, int32_t into = -1,
+                    const int32_t *kids = nullptr, int32_t parent = -1, int shared = 0);
+    void check_room(const Entry &e, int32_t n) const {
+        const int64_t most = cfg.max_tokens ? cfg.max_tokens : (int64_t)table_ld * PC_PAGE;
+        if (n < 0 || (int64_t)e.len + n > most) throw Error("prompt cache: an entry holds at most " + std::to_string(most) + " tokens");
+    }
+    // the pages that n more tokens of an entry need, fit for use on `stream`
+    std::vector<int32_t> pages_for(Entry &e, int32_t n, void *stream) {
+        const int have = (int)e.pages.size(), need = (int)(((int64_t)e.len + n + PC_PAGE - 1) / PC_PAGE);
+        if (need <= have) return {};
+        std::vector<int32_t> got = pick_pages(need - have, stream);
+        if (stream != e.home) {          // (its table may be in use on the home stream)
+            wait_all();
+            e.foreign = true;
+        }
+        return got;
+    }
+    void grow(Entry &e, int32_t n, const std::vector<int32_t> &got) {
+        for (int32_t p : got) { take(p); e.pages.push_back(p); }
+        e.len += n;
+    }
     void set_table(int32_t e, int at_, const int32_t *val, int n, hipStream_t st);
     void remap(const int32_t *src, const int32_t *dst, int n, hipStream_t st);
 };
 
-void mi_prompt_cache::copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st) {
+void mi_prompt_cache::copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st, int32_t into,
+                                 const int32_t *kids, int32_t parent, int shared) {
     PcCopyArgs a{};
     a.from = from; a.to = to; a.page_stride = page_stride; a.segs = cfg.n_layers * cfg.n_kv_heads * 2; a.hd = cfg.head_dim; a.rows = rows;
+    a.tables = tables.get<int32_t>(); a.ld = table_ld; a.shared = shared;
+    if (kids) a.parent_table = table(parent);
+    constexpr int most = sizeof a.src / sizeof a.src[0];
     const int64_t words = (int64_t)a.segs * rows * cfg.head_dim / 8;
-    for (int j0 = 0; j0 < n; j0 += 480) {
-        const int m = std::min(480, n - j0);
+    for (int j0 = 0; j0 < n; j0 += most) {
+        const int m = std::min(most, n - j0);
         std::copy(src + j0, src + j0 + m, a.src);
         std::copy(dst + j0, dst + j0 + m, a.dst);
+        if (kids) std::copy(kids + j0, kids + j0 + m, a.kid);
+        if (into >= 0) a.entry_table = table(into) + j0;
         hipLaunchKernelGGL(pc_copy_kernel, dim3((unsigned)((words + 1023) / 1024), (unsigned)m), dim3(256), 0, st, a);
         MI_HIP(hipGetLastError());
     }
@@ -132,6 +178,26 @@ void mi_prompt_cache::remap(const int32_t *src, const int32_t *dst, int n, hipSt
 
 namespace {
 
+// memory that a kernel on `device` may use
+bool on_device(const void *p, int device) {
+    hipPointerAttribute_t attr;
+    if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return attr.type == hipMemoryTypeManaged || (attr.type == hipMemoryTypeDevice && attr.device == device);
+}
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+void check_strides(const mi_prompt_cache *c, int n, const void *k, const int64_t *ks, const void *v, const int64_t *vs) {
+    MI_REQUIRE(aligned16(k) && aligned16(v), "prompt cache: keys and values must be 16-byte aligned");
+    MI_REQUIRE(!n || (on_device(k, c->device) && on_device(v, c->device)), "prompt cache: memory of the cache's device only");
+    for (int i = 0; i < 3; ++i) MI_REQUIRE(ks[i] % 8 == 0 && vs[i] % 8 == 0, "prompt cache: strides must be multiples of 8 elements");
+}
+void write_sources(PcWriteArgs &a, const void *k, const int64_t *ks, const void *v, const int64_t *vs) {
+    a.k = static_cast<const bf16_t *>(k); a.k_layer = ks[0]; a.k_token = ks[1]; a.k_head = ks[2];
+    a.v = static_cast<const bf16_t *>(v); a.v_layer = vs[0]; a.v_token = vs[1]; a.v_head = vs[2]; a.v_dim = 1;
+}
 void write_args(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n, PcWriteArgs &a, void *stream) {
     Entry &e = c->at(entry);
     MI_REQUIRE(layer >= 0 && n_layers >= 1 && n_layers <= c->cfg.n_layers - layer, "prompt cache: layer out of range");
@@ -149,17 +215,6 @@ void write_launch(const PcWriteArgs &a, void *stream) {
     hipLaunchKernelGGL(pc_write_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), a);
     MI_HIP(hipGetLastError());
 }
-
-// memory that a kernel on `device` may use
-bool on_device(const void *p, int device) {
-    hipPointerAttribute_t attr;
-    if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
-        (void)hipGetLastError();
-        return false;
-    }
-    return attr.type == hipMemoryTypeManaged || (attr.type == hipMemoryTypeDevice && attr.device == device);
-}
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // checks what the kernels take for granted, and fills in their arguments
 PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const PromptForms &f) {
@@ -306,7 +361,7 @@ int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pag
         MI_HIP(hipDeviceSynchronize());
         c->ref.assign(g.n_pages, 0);
         c->tag.assign(g.n_pages, ANY);
-        for (int32_t p = 0; p < g.n_pages; ++p) c->free_pages.insert(c->free_pages.end(), p);
+        c->free_pages.reset(g.n_pages, 0);
         c->entries.resize(g.max_entries);
         *out = c.release();
     });
@@ -340,19 +395,38 @@ int mi_prompt_cache_reserve(mi_prompt_cache *c, int32_t entry, int32_t n, void *
         std::lock_guard<std::mutex> lk(c->mu);
         MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot grow while the stream is captured");
         Entry &e = c->at(entry);
-        const int64_t max_tokens = c->cfg.max_tokens ? c->cfg.max_tokens : (int64_t)c->table_ld * PC_PAGE;
-        MI_REQUIRE(n >= 0 && (int64_t)e.len + n <= max_tokens, "prompt cache: an entry holds at most " + std::to_string(max_tokens) + " tokens");
-        const int have = (int)e.pages.size(), need = (int)(((int64_t)e.len + n + PC_PAGE - 1) / PC_PAGE);
-        if (need > have) {
-            const std::vector<int32_t> got = c->pick_pages(need - have, stream);
-            if (stream != e.home) {      // (its table may be in use on the home stream)
-                c->wait_all();
-                e.foreign = true;
-            }
-            c->set_table(entry, have, got.data(), need - have, as_stream(stream));
-            for (int32_t p : got) { c->take(p); e.pages.push_back(p); }
+        c->check_room(e, n);
+        const std::vector<int32_t> got = c->pages_for(e, n, stream);
+        if (!got.empty()) c->set_table(entry, (int)e.pages.size(), got.data(), (int)got.size(), as_stream(stream));
+        c->grow(e, n, got);
+    });
+}
+
+int mi_prompt_cache_extend(mi_prompt_cache *c, int32_t entry, int32_t n, const void *k, const int64_t ks[3], const void *v, const int64_t vs[3],
+                           void *stream) {
+    return guard([&] {
+        MI_REQUIRE(c && ks && vs && (!n || (k && v)), "null argument");
+        DeviceGuard dg(c->device);
+        std::lock_guard<std::mutex> lk(c->mu);
+        MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot grow while the stream is captured");
+        Entry &e = c->at(entry);
+        c->check_room(e, n);
+        check_strides(c, n, k, ks, v, vs);
+        const int start = e.len, have = (int)e.pages.size();
+        const std::vector<int32_t> got = c->pages_for(e, n, stream);
+        PcWriteArgs a{};
+        const int first = start / PC_PAGE, touched = have + (int)got.size() - first;
+        if (touched <= (int)(sizeof a.pages_of / sizeof a.pages_of[0])) {   // one launch: the pages' numbers go with it
+            std::copy(e.pages.begin() + first, e.pages.end(), a.pages_of);
+            std::copy(got.begin(), got.end(), a.pages_of + have - first);
+            a.n_pages = touched; a.n_new = (int)got.size(); a.new_at = c->table(entry) + have;
+        } else {
+            c->set_table(entry, have, got.data(), (int)got.size(), as_stream(stream));
         }
-        e.len += n;
+        c->grow(e, n, got);
+        write_args(c, entry, 0, c->cfg.n_layers, start, n, a, stream);
+        write_sources(a, k, ks, v, vs);
+        write_launch(a, stream);
     });
 }
 
@@ -362,18 +436,15 @@ int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int3
         MI_REQUIRE(c && ks && vs && (!n || (k && v)), "null argument");
         DeviceGuard dg(c->device);
         std::lock_guard<std::mutex> lk(c->mu);
-        MI_REQUIRE(aligned16(k) && aligned16(v), "prompt cache: keys and values must be 16-byte aligned");
-        MI_REQUIRE(!n || (on_device(k, c->device) && on_device(v, c->device)), "prompt cache: memory of the cache's device only");
-        for (int i = 0; i < 3; ++i) MI_REQUIRE(ks[i] % 8 == 0 && vs[i] % 8 == 0, "prompt cache: strides must be multiples of 8 elements");
+        check_strides(c, n, k, ks, v, vs);
         PcWriteArgs a{};
         write_args(c, entry, layer, n_layers, start, n, a, stream);
-        a.k = static_cast<const bf16_t *>(k); a.k_layer = ks[0]; a.k_token = ks[1]; a.k_head = ks[2];
-        a.v = static_cast<const bf16_t *>(v); a.v_layer = vs[0]; a.v_token = vs[1]; a.v_head = vs[2]; a.v_dim = 1;
+        write_sources(a, k, ks, v, vs);
         write_launch(a, stream);
     });
 }
 
-int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *out, void *stream) {
+int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *out, int32_t *page, void *stream) {
     return guard([&] {
         MI_REQUIRE(c && (out || !count), "null argument");
         MI_REQUIRE(count >= 0, "prompt cache: negative count");
@@ -386,24 +457,27 @@ int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32
         const int rows = e.len % PC_PAGE, shared = e.len / PC_PAGE;
         const std::vector<int32_t> own = rows ? c->pick_pages(count, stream) : std::vector<int32_t>();
         hipStream_t st = as_stream(stream);
-        PcForkArgs a{};
-        a.tables = c->tables.get<int32_t>(); a.ld = c->table_ld; a.parent = entry; a.shared = shared;
-        if (!e.pages.empty())
+        if (rows) {
+            const std::vector<int32_t> src(count, e.pages[shared]);
+            c->copy_pages(c->pages, c->pages, src.data(), own.data(), count, rows, st, -1, kids.data(), entry, shared);
+        } else if (shared) {
+            PcForkArgs a{};
+            a.tables = c->tables.get<int32_t>(); a.ld = c->table_ld; a.parent = entry; a.shared = shared;
             for (int j0 = 0; j0 < count; j0 += 480) {
                 a.n = std::min(480, count - j0);
-                for (int j = 0; j < a.n; ++j) { a.entry[j] = kids[j0 + j]; a.own[j] = rows ? own[j0 + j] : -1; }
+                std::copy(kids.begin() + j0, kids.begin() + j0 + a.n, a.entry);
                 hipLaunchKernelGGL(pc_fork_kernel, dim3((unsigned)a.n), dim3(256), 0, st, a);
                 MI_HIP(hipGetLastError());
             }
-        if (rows) {
-            const std::vector<int32_t> src(count, e.pages[shared]);
-            c->copy_pages(c->pages, c->pages, src.data(), own.data(), count, rows, st);
         }
         c->reads(e, stream, false);
         const std::vector<int32_t> base(e.pages.begin(), e.pages.begin() + shared);
+        for (int32_t p : base) c->ref[p] += count;
         for (int j = 0; j < count; ++j) {
-            std::vector<int32_t> pg = base;
-            for (int32_t p : base) ++c->ref[p];
+            std::vector<int32_t> pg;
+            pg.reserve(base.size() + 1);
+            pg = base;
+            if (page) page[j] = rows ? own[j] : -1;
             if (rows) { c->take(own[j]); pg.push_back(own[j]); }
             c->open(kids[j], c->entries[entry].len, std::move(pg), stream);
             out[j] = kids[j];
@@ -421,8 +495,7 @@ int mi_prompt_cache_copy(mi_prompt_cache *c, int32_t entry, int32_t *copy, void 
         const int n = (int)e.pages.size();
         const int32_t to = c->pick_entries(1, stream)[0];
         std::vector<int32_t> own = c->pick_pages(n, stream);
-        c->set_table(to, 0, own.data(), n, as_stream(stream));
-        c->copy_pages(c->pages, c->pages, e.pages.data(), own.data(), n, PC_PAGE, as_stream(stream));
+        c->copy_pages(c->pages, c->pages, e.pages.data(), own.data(), n, PC_PAGE, as_stream(stream), to);
         c->reads(e, stream, false);
         for (int32_t p : own) c->take(p);
         c->open(to, e.len, std::move(own), stream);
@@ -437,10 +510,11 @@ int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *list, voi
         std::lock_guard<std::mutex> lk(c->mu);
         MI_REQUIRE(!capturing(stream), "prompt cache: entries cannot be freed while the stream is captured");
         bool wait = false;
-        std::set<int32_t> seen;
+        std::vector<bool> seen(c->entries.size());
         for (int32_t i = 0; i < n; ++i) {
             const Entry &e = c->at(list[i]);
-            MI_REQUIRE(seen.insert(list[i]).second, "prompt cache: an entry is freed twice");
+            if (seen[list[i]]) throw Error("prompt cache: an entry is freed twice");
+            seen[list[i]] = true;
             wait = wait || e.foreign || e.home != stream;
         }
         if (wait) c->wait_all();
@@ -463,12 +537,12 @@ int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
         DeviceGuard dg(c->device);
         std::lock_guard<std::mutex> lk(c->mu);
         MI_REQUIRE(!capturing(stream), "prompt cache: pages cannot be moved while the stream is captured");
-        const int32_t n = c->cfg.n_pages, used = n - (int32_t)c->free_pages.size();
+        const int32_t n = c->cfg.n_pages, used = n - c->free_pages.count;
         std::vector<int32_t> dst, src;
-        for (int32_t p : c->free_pages) {
-            if (p >= used) break;
-            dst.push_back(p);
-        }
+        c->free_pages.each([&](int32_t p) {
+            if (p < used) dst.push_back(p);
+            return p < used;
+        });
         for (int32_t p = used; p < n && src.size() < dst.size(); ++p)
             if (c->ref[p]) src.push_back(p);
         if (moved) *moved = (int32_t)src.size();
@@ -524,8 +598,7 @@ int mi_prompt_cache_resize(mi_prompt_cache *c, void *pages, int32_t n_pages, voi
             for (int32_t &p : e.pages) p = to[p];
         c->ref = std::move(ref);
         c->tag.assign(n_pages, ANY);
-        c->free_pages.clear();
-        for (int32_t p = (int32_t)src.size(); p < n_pages; ++p) c->free_pages.insert(c->free_pages.end(), p);
+        c->free_pages.reset(n_pages, (int)src.size());
         c->pages = static_cast<bf16_t *>(pages);
         c->cfg.n_pages = n_pages;
         std::swap(c->own.p, own.p);
@@ -548,7 +621,7 @@ int mi_prompt_cache_used(mi_prompt_cache *c, int32_t *used_pages, int32_t *entri
     return guard([&] {
         MI_REQUIRE(c, "null argument");
         std::lock_guard<std::mutex> lk(c->mu);
-        if (used_pages) *used_pages = c->cfg.n_pages - (int32_t)c->free_pages.size();
+        if (used_pages) *used_pages = c->cfg.n_pages - c->free_pages.count;
         if (entries) *entries = (int32_t)std::count_if(c->entries.begin(), c->entries.end(), [](const Entry &e) { return e.live; });
     });
 }

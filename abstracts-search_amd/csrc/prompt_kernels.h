@@ -657,8 +657,15 @@ struct PcWriteArgs {
     int64_t page_stride, layer_stride;
     const int32_t *table;
     int layer, n_layers, start, n, n_kv, hd, k_inter;
+    // pages of the tokens' positions, from start / 64 on, where they travel with the launch: the last n_new of them are new, and the
+    // first workgroup enters them in the table (n_pages = 0: the table holds them all)
+    int n_pages, n_new;
+    int32_t *new_at;
+    int32_t pages_of[896];
 };
 __global__ void __launch_bounds__(256) pc_write_kernel(PcWriteArgs a) {
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.n_new; i += 256) a.new_at[i] = a.pages_of[a.n_pages - a.n_new + i];
     const int per = a.hd / 8;
     const int64_t total = (int64_t)a.n_layers * a.n * a.n_kv * per * 2;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -671,7 +678,7 @@ __global__ void __launch_bounds__(256) pc_write_kernel(PcWriteArgs a) {
     r /= a.n;
     const int which = (int)(r & 1), l = (int)(r >> 1);
     const int pos = a.start + t;
-    bf16_t *dst = a.pages + a.table[pos / PC_PAGE] * a.page_stride + (a.layer + l) * a.layer_stride +
+    bf16_t *dst = a.pages + (a.n_pages ? a.pages_of[pos / PC_PAGE - a.start / PC_PAGE] : a.table[pos / PC_PAGE]) * a.page_stride + (a.layer + l) * a.layer_stride +
                   (((int64_t)h * 2 + which) * PC_PAGE + pos % PC_PAGE) * a.hd + c * 8;
     const bf16_t *src = which ? a.v + l * a.v_layer + t * a.v_token + h * a.v_head : a.k + l * a.k_layer + t * a.k_token + h * a.k_head;
     if (which ? a.v_dim == 1 : !a.k_inter) {
@@ -690,9 +697,22 @@ struct PcCopyArgs {
     bf16_t *to;
     int64_t page_stride;                  // elements
     int segs, hd, rows;                   // segments of a page: layers x key heads x 2
-    int32_t src[480], dst[480];
+    // the tables of what is copied, written by the first workgroup of each job: `entry_table` [job] = dst (one entry's pages), or the
+    // table of the job's own new entry, which begins with the first `shared` pages of parent_table (tables + kid * ld)
+    int32_t *entry_table, *tables;
+    const int32_t *parent_table;
+    int64_t ld;
+    int shared;
+    int32_t src[320], dst[320], kid[320];
 };
 __global__ void __launch_bounds__(256) pc_copy_kernel(PcCopyArgs a) {
+    if (blockIdx.x == 0) {
+        if (a.entry_table && threadIdx.x == 0) a.entry_table[blockIdx.y] = a.dst[blockIdx.y];
+        if (a.parent_table) {
+            int32_t *t = a.tables + a.kid[blockIdx.y] * a.ld;
+            for (int i = threadIdx.x; i <= a.shared; i += 256) t[i] = i < a.shared ? a.parent_table[i] : a.dst[blockIdx.y];
+        }
+    }
     const int per = a.rows * a.hd / 8;                        // 16-byte words of a segment
     const int64_t total = (int64_t)a.segs * per;
     const bf16_t *s = a.from + a.src[blockIdx.y] * a.page_stride;
@@ -703,18 +723,17 @@ __global__ void __launch_bounds__(256) pc_copy_kernel(PcCopyArgs a) {
     }
 }
 
-// the tables of new entries that begin as `parent` does: its first `shared` pages, then (own[i] >= 0) one page of the entry's own
+// the tables of new entries that begin as `parent` does, its pages all full
 struct PcForkArgs {
     int32_t *tables;
     int64_t ld;
     int parent, shared, n;
-    int32_t entry[480], own[480];
+    int32_t entry[480];
 };
 __global__ void __launch_bounds__(256) pc_fork_kernel(PcForkArgs a) {
     const int32_t *p = a.tables + a.parent * a.ld;
     int32_t *t = a.tables + a.entry[blockIdx.x] * a.ld;
     for (int i = threadIdx.x; i < a.shared; i += 256) t[i] = p[i];
-    if (threadIdx.x == 0 && a.own[blockIdx.x] >= 0) t[a.shared] = a.own[blockIdx.x];
 }
 
 // page numbers src[j] -> dst[j] in every table (src ascending; words behind an entry's length may change too, nothing reads them)

@@ -31,6 +31,7 @@ class _Cfg(ctypes.Structure):
     _fields_ = [(n, c_int32) for n in ("n_layers", "n_kv_heads", "head_dim", "dtype", "n_pages", "max_entries", "max_tokens")]
 
 
+_Strides = c_int64 * 3
 # mi_prompt_attn, field by field
 _ATTN = struct.Struct("@6i4P8q2PifiiPq")
 
@@ -50,7 +51,8 @@ class _Lib:
                 "mi_prompt_cache_new": [v, v, pi32],
                 "mi_prompt_cache_reserve": [v, i32, i32, v],
                 "mi_prompt_cache_write": [v, i32, i32, i32, i32, i32, v, POINTER(c_int64), v, POINTER(c_int64), v],
-                "mi_prompt_cache_fork": [v, i32, i32, pi32, v],
+                "mi_prompt_cache_extend": [v, i32, i32, v, POINTER(c_int64), v, POINTER(c_int64), v],
+                "mi_prompt_cache_fork": [v, i32, i32, pi32, pi32, v],
                 "mi_prompt_cache_copy": [v, i32, pi32, v],
                 "mi_prompt_cache_free": [v, i32, pi32, v],
                 "mi_prompt_cache_compact": [v, v, pi32],
@@ -115,6 +117,8 @@ class PromptCache:
         self._close = weakref.finalize(self, _destroy, self._h)
         self._lib = lib
         self._table_cap = -(-max_tokens // PAGE) if max_tokens else n_pages   # pages of the longest entry
+        self._tables: dict = {}                      # entry -> its table, as far as known: a list, or (full pages, the last one)
+        self._moves = 0                              # how often pages have moved
         self._plans: dict = {}                       # (entry, shapes) -> bytes of workspace, until an entry changes
         # torch's current stream as a pointer (building the Stream object first is 1.7 us of a 10 us call)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -131,13 +135,14 @@ class PromptCache:
     def reserve(self, entry: int, n: int) -> None:
         """n more tokens at the end of the entry, to be filled by ``write``"""
         self._plans.clear()
+        self._tables.pop(entry, None)
         _check(self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream()))
 
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
         """keys and values of tokens start .. of layers layer ..: [layers, n, n_kv_heads, head_dim], or one layer without the
         first axis.  Tokens in pages that other entries share are refused."""
         k, v = self._kv(k, v)
-        ks, vs = (c_int64 * 3)(*k.stride()[:3]), (c_int64 * 3)(*v.stride()[:3])
+        ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
         _check(self._lib.mi_prompt_cache_write(self._h, entry, layer, k.shape[0], start, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs,
                                                self._stream()))
 
@@ -146,9 +151,10 @@ class PromptCache:
         k, v = self._kv(k, v)
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
-        start = self.length(entry)
-        self.reserve(entry, k.shape[1])
-        self.write(entry, k, v, start)
+        self._plans.clear()
+        self._tables.pop(entry, None)
+        ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
+        _check(self._lib.mi_prompt_cache_extend(self._h, entry, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs, self._stream()))
 
     def _kv(self, k, v):
         if k.dim() == 3 and v.dim() == 3:
@@ -170,9 +176,17 @@ class PromptCache:
         """`count` new entries that begin as `entry` does: its full pages are shared, the tokens of its last page copied"""
         if count < 0:
             raise ValueError(f"PromptCache.fork: count must not be negative, got {count}")
-        out = (c_int32 * count)()
-        _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, self._stream()))
-        return list(out)
+        out, own, moves = (c_int32 * count)(), (c_int32 * count)(), self._moves
+        _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, own, self._stream()))
+        kids, own = out[:], own[:]
+        if count > 1:                                # (their tables without asking for each of them)
+            full = self.table(entry)
+            if own[0] >= 0:
+                full.pop()
+            known = {k: (full, p) for k, p in zip(kids, own)}
+            if moves == self._moves:
+                self._tables.update(known)
+        return kids
 
     def copy(self, entry: int) -> int:
         """a new entry with the same tokens in pages of its own"""
@@ -184,12 +198,18 @@ class PromptCache:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
         self._plans.clear()
+        for e in entries:
+            self._tables.pop(e, None)
         _check(self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream()))
 
     def compact(self) -> int:
         """moves pages down until the used ones are the first ones of the pool; how many were moved"""
         n = c_int32()
+        self._moves += 1
+        self._tables.clear()
         _check(self._lib.mi_prompt_cache_compact(self._h, self._stream(), ctypes.byref(n)))
+        self._moves += 1
+        self._tables.clear()
         return n.value
 
     def resize(self, n_pages: int) -> None:
@@ -199,7 +219,11 @@ class PromptCache:
         if n_pages < 1:
             raise ValueError(f"PromptCache.resize: n_pages must be positive, got {n_pages}")
         pages = torch.zeros((n_pages, *self.pages.shape[1:]), dtype=self.dtype, device=self.device)
+        self._moves += 1
+        self._tables.clear()
         _check(self._lib.mi_prompt_cache_resize(self._h, pages.data_ptr(), n_pages, self._stream()))
+        self._moves += 1
+        self._tables.clear()
         self.pages = pages
 
     # -- what is held -----------------------------------------------------------
@@ -210,6 +234,10 @@ class PromptCache:
 
     def table(self, entry: int) -> list[int]:
         """the page numbers of the entry, in order"""
+        known = self._tables.get(entry)
+        if known is not None:
+            full, last = known
+            return full + [last] if last >= 0 else full[:]
         cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
         _check(self._lib.mi_prompt_cache_entry(self._h, entry, ctypes.byref(n), t, cap))

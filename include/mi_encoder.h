@@ -166,8 +166,12 @@ int mi_prompt_cache_reserve(mi_prompt_cache *c, int32_t entry, int32_t n, void *
  * multiples of 8; pointers 16-byte aligned).  Pages that other entries share are refused. */
 int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n,
                           const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3], void *stream);
-/* count new entries that begin as `entry` does: full pages are shared, the used rows of the last page are copied. */
-int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *entries, void *stream);
+/* n more tokens and their keys and values, all layers, in one launch: reserve and write. */
+int mi_prompt_cache_extend(mi_prompt_cache *c, int32_t entry, int32_t n, const void *k, const int64_t k_strides[3], const void *v,
+                           const int64_t v_strides[3], void *stream);
+/* count new entries that begin as `entry` does: full pages are shared, the used rows of the last page are copied.  pages (may be
+ * NULL): the number of each one's own last page, -1 where all pages are full. */
+int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *entries, int32_t *pages, void *stream);
 /* one new entry with pages of its own throughout. */
 int mi_prompt_cache_copy(mi_prompt_cache *c, int32_t entry, int32_t *copy, void *stream);
 int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *entries, void *stream);

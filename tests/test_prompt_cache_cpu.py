@@ -40,7 +40,7 @@ def test_c_entries_refuse_null_and_bad_arguments(pc):
         assert b"prompt cache" in lib.mi_enc_last_error()
     assert lib.mi_prompt_cache_new(None, None, ctypes.byref(n)) != 0
     assert lib.mi_prompt_cache_reserve(None, 0, 1, None) != 0
-    assert lib.mi_prompt_cache_fork(None, 0, 1, ctypes.byref(n), None) != 0
+    assert lib.mi_prompt_cache_fork(None, 0, 1, ctypes.byref(n), None, None) != 0
     assert lib.mi_prompt_cache_free(None, 0, None, None) != 0
     assert lib.mi_prompt_cache_compact(None, None, None) != 0
     assert lib.mi_prompt_cache_resize(None, None, 1, None) != 0
