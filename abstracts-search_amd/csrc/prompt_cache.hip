@@ -271,9 +271,11 @@ Plan plan_of(const PromptArgs &a, int hd) {
 template <class T, int HD, bool VT>
 void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)p.tiles * p.splits * a.n_kv + 7) / 8 * 8));
-    if (p.nw == 1) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT>), grid, dim3(64), 0, st, a);
-    else if (p.nw == 2) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT>), grid, dim3(128), 0, st, a);
-    else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT>), grid, dim3(256), 0, st, a);
+    // few rows: the probabilities in two parts (see the kernel)
+    if (p.nw == 1) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT, true>), grid, dim3(64), 0, st, a);
+    else if (p.nw == 2) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT, true>), grid, dim3(128), 0, st, a);
+    else if (p.rows <= 4096) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT, false>), grid, dim3(256), 0, st, a);
     MI_HIP(hipGetLastError());
     if (p.splits > 1) {
         constexpr int per_wg = 256 / (HD / 4);                                    // groups of lanes

@@ -54,6 +54,7 @@ struct TBf16 {
     }
     __device__ static float up(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
     __device__ static unsigned pack(float lo, float hi) { return pack2(lo, hi); }
+    __device__ static unsigned scaled(unsigned two, float f) { return pack(up((unsigned short)(two & 0xffffu)) * f, up((unsigned short)(two >> 16)) * f); }
     __device__ static unsigned short down(float v) { return (unsigned short)(pack2(v, v) & 0xffffu); }
     // probabilities are rounded to the values' type for the product with V (relative error 2^-9 each, the denominator sums the
     // f32 values); bf16 has f32's exponents
@@ -69,6 +70,7 @@ struct TF16 {
         const f32x2_t v = {lo, hi};
         return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2_t));
     }
+    __device__ static unsigned scaled(unsigned two, float f) { return pack(up((unsigned short)(two & 0xffffu)) * f, up((unsigned short)(two >> 16)) * f); }
     __device__ static unsigned short down(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
     // f16 loses what is below 2^-25: the probabilities are held as 2^7 p (p <= 1), so that a long tail of small ones keeps its
     // weight; the factor cancels in o / sum
@@ -309,9 +311,13 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
     }
 }
 
+// TWO: the probabilities enter the product with V in two parts (what the type holds of them, and of the rest), which leaves the
+// output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output.  Few rows are
+// bound by latency or by reading the pages and take the second product for nothing (one query 9.3 us either way, four tokens
+// behind 65 500 61); many rows are bound by the products.
 // Two stages of LDS, so that two workgroups share a CU and overlap each other (four stages and one workgroup a CU: 88 us instead
 // of 52 on four tokens behind 65 500, 1026 instead of 1005 on 12.7 k tokens behind 4096).
-template <class T, int HD, int NW, bool VT>
+template <class T, int HD, int NW, bool VT, bool TWO>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
     constexpr int KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
     constexpr int RPP = 64 / SL, PIECES = KC / RPP, PPW = PIECES / NW;            // rows of a 1-KiB piece, pieces of a K or V tile, of a wave
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
         const lds_t *Ks = smem + (i % NS) * STG, *Vs = Ks + KC * HD;
         constexpr int EPS = 16 / NKK;                                            // exponentials of a slot (both phases have NKK slots a tile)
         static_assert(2 * NDT == NKK, "as many products of V as of K");
-        u32x4 kf[4], vf[4], pf[4];                                               // fragments in flight; probabilities, packed: keys 16 J + 8 half ..
+        u32x4 kf[4], vf[4], pf[4], pr[TWO ? 4 : 1];                              // fragments in flight; probabilities, packed: keys 16 J + 8 half .., and their rest
         f32x16 s[2];
         const bool own = i >= np;
         const int b = base_of(i), l = own ? lo - b : 0, h = (own ? hi : a.P) - b;   // the row sees keys [l, h) of the chunk
@@ -513,8 +519,10 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            pf[q][e] = T::pack(T::up((unsigned short)(pf[q][e] & 0xffffu)) * alpha, T::up((unsigned short)(pf[q][e] >> 16)) * alpha);
+                        for (int e = 0; e < 4; ++e) {
+                            pf[q][e] = T::scaled(pf[q][e], alpha);
+                            if constexpr (TWO) pr[q][e] = T::scaled(pr[q][e], alpha);
+                        }
                 }
             }
             sub = (mrow == -__builtin_huge_valf() ? 0.f : mrow) - T::shift;
@@ -530,6 +538,11 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
                     unsigned two = T::pack(s[j][r - 1], s[j][r]);
                     asm volatile("" : "+v"(two), "+v"(sum[0]), "+v"(sum[1]));    // (here, not where it is used: the compiler sinks it past the products)
                     pf[2 * j + r / 8][r / 2 % 4] = two;
+                    if constexpr (TWO) {
+                        unsigned rest = T::pack(s[j][r - 1] - T::up((unsigned short)(two & 0xffffu)), s[j][r] - T::up((unsigned short)(two >> 16)));
+                        asm volatile("" : "+v"(rest));
+                        pr[2 * j + r / 8][r / 2 % 4] = rest;
+                    }
                 }
             }
         };
@@ -555,6 +568,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
 #pragma unroll
         for (int g = 0; g < NKK; ++g) {
             o[g % NDT] = T::mfma(vf[g & 3], pf[g / NDT], o[g % NDT]);
+            if constexpr (TWO) o[g % NDT] = T::mfma(vf[g & 3], pr[g / NDT], o[g % NDT]);
             read_v(g + 4);
             exps(std::integral_constant<int, 1>{}, g);
             __builtin_amdgcn_sched_barrier(0);
@@ -563,6 +577,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
 #pragma unroll
         for (int g = NKK; g < 2 * NKK; ++g) {
             o[g % NDT] = T::mfma(vf[g & 3], pf[g / NDT], o[g % NDT]);
+            if constexpr (TWO) o[g % NDT] = T::mfma(vf[g & 3], pr[g / NDT], o[g % NDT]);
             if (g + 4 < 2 * NKK) read_v(g + 4);
             __builtin_amdgcn_sched_barrier(0);
         }
