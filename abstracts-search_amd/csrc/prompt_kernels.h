@@ -114,7 +114,9 @@ __device__ __forceinline__ int quotient(int n, int d, float r) {
 
 // the text of token t, and the keys [lo, hi) of its own that it sees; t behind the last text: false.  Whatever the two arrays
 // hold, the result stays inside [0, n_keys].
-__device__ __forceinline__ bool prompt_own_range(const PromptArgs &a, const int *cu_q, const int *cu_k, int t, int &lo, int &hi) {
+// (Ints: a pointer into global memory or into LDS -- one that may be either would be read by flat instructions, whose waits are for both)
+template <class Ints>
+__device__ __forceinline__ bool prompt_own_range(const PromptArgs &a, Ints cu_q, Ints cu_k, int t, int &lo, int &hi) {
     int q0 = 0, q1 = a.n_tokens, k0 = 0, k1 = a.n_keys;
     if (a.cu_q) {
         int i = 0, n = a.n_texts;                             // the last text with cu_q[i] <= t
@@ -431,11 +433,17 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
     const int early = min(np, NS);
     for (int i = 0; i < early; ++i) issue(i);
     if (in_lds) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int *cq = in_lds ? s_cu[0] : a.cu_q, *ck = in_lds ? s_cu[1] : a.cu_k;
     // one search for all: lanes 0 .. 31 for their rows, lane 32 for the tile's first token, the others for the last one that belongs to a text
-    const int t_end = min(a.cu_q ? min(cq[a.n_texts], a.n_tokens) : a.n_tokens, quotient(min(r0 + 32 * NW, rows) - 1, a.G, a.r_G) + 1);
     int lo, hi;
-    bool live = prompt_own_range(a, cq, ck, half ? (li ? t_end - 1 : quotient(r0, a.G, a.r_G)) : token, lo, hi);
+    bool live;
+    const int t_last = quotient(min(r0 + 32 * NW, rows) - 1, a.G, a.r_G), t_first = quotient(r0, a.G, a.r_G);
+    auto search = [&](auto cu_q, auto cu_k) {
+        const int end = a.cu_q ? min(cu_q[a.n_texts] - 1, t_last) : t_last;
+        live = prompt_own_range(a, cu_q, cu_k, half ? (li ? end : t_first) : token, lo, hi);
+    };
+    typedef const __attribute__((address_space(3))) int *lds_ints;
+    if (in_lds) search((lds_ints)s_cu[0], (lds_ints)s_cu[1]);
+    else search(a.cu_q, a.cu_k);
     const uint64_t found = __builtin_amdgcn_ballot_w64(live);
     k0 = __builtin_amdgcn_readlane(lo, 32);
     k1 = __builtin_amdgcn_readlane(hi, 33);

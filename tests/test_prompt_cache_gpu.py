@@ -396,6 +396,90 @@ def test_strided_keys_and_values_are_stored(pc):
     assert torch.equal(cache.pages[1][:, :, 0, 6:11].transpose(1, 2), odd)
 
 
+def test_more_pages_than_a_launch_carries(pc):
+    """prompts of more than 896 pages, forks of more than 320 entries, copies and moves of more than 480 pages: several launches each"""
+    cache = pc.PromptCache(1, 1, 64, 4000, max_entries=800)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = 64 * 1000 + 7
+    k, v = (torch.randn(1, n, 1, 64, generator=g, device="cuda").to(BF) for _ in range(2))
+    low, e = cache.new(), cache.new()
+    cache.extend(low, k[:, :64 * 900], v[:, :64 * 900])
+    cache.extend(e, k[:, :5], v[:, :5])
+    cache.extend(e, k[:, 5:], v[:, 5:])                          # 1001 pages, the first one begun
+    kids = cache.fork(e, 700)
+    cache.free(low)
+    assert cache.compact() == 900 and cache.used_pages == 1701
+
+    def holds(x):
+        t = torch.tensor(cache.table(x), device="cuda")
+        return [cache.pages[t, 0, 0, w].reshape(-1, 64)[:n] for w in (0, 1)]
+
+    for x in (e, kids[0], kids[319], kids[320], kids[699], cache.copy(kids[5])):
+        assert torch.equal(holds(x)[0], k[0, :, 0]) and torch.equal(holds(x)[1], v[0, :, 0])
+    q = torch.randn(3, 2, 64, generator=g, device="cuda").to(BF)
+    none = torch.zeros(0, 1, 64, dtype=BF, device="cuda")
+    o, b = reference_many(q, k[0], v[0], none, none, [0, 3], [0, 0], True)
+    for x in (e, kids[650]):
+        close(cache.attention(x, 0, q), o, b)
+    cache.resize(3000)
+    assert torch.equal(holds(kids[650])[0], k[0, :, 0])
+    close(cache.attention(kids[650], 0, q), o, b)
+
+
+def test_offsets_beyond_32_bits(pc):
+    """a pool of 5 GiB: entries behind the first 4 GiB (bytes, and 2^31 elements)"""
+    layers, kv, hd = 16, 4, 128                                  # 2 MiB a page
+    cache = pc.PromptCache(layers, kv, hd, 2600)
+    low = cache.new()
+    cache.reserve(low, 64 * 2300)                                # 4.6 GiB
+    g = torch.Generator(device="cuda").manual_seed(9)
+    k, v = (torch.randn(layers, 200, kv, hd, generator=g, device="cuda").to(BF) for _ in range(2))
+    e = cache.new()
+    cache.extend(e, k, v)
+    assert min(cache.table(e)) == 2300
+    kid = cache.fork(e)[0]
+    q = torch.randn(9, 8, hd, generator=g, device="cuda").to(BF)
+    none = torch.zeros(0, kv, hd, dtype=BF, device="cuda")
+    for x in (e, kid, cache.copy(e)):
+        for layer in (0, layers - 1):
+            o, b = reference_many(q, k[layer], v[layer], none, none, [0, 9], [0, 0], True)
+            close(cache.attention(x, layer, q), o, b)
+    cache.free(low)
+    assert cache.compact() == cache.used_pages
+    close(cache.attention(kid, layers - 1, q), o, b)
+
+
+def test_nothing_to_see_and_broadcast_operands(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 6, 3, 64, 0, [4, 9])
+    assert (cache.attention(e, 1, q) == 0).all()
+    none = torch.zeros(0, 3, 64, dtype=BF, device="cuda")
+    assert (cache.attention(e, 1, q, none, none, dev(cu_q), dev([0, 0, 0]), causal=False) == 0).all()
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 6, 3, 64, 66, [4, 9])
+    k1, v1 = k[:, :1].expand(-1, 3, -1), v[:, :1].expand(-1, 3, -1)              # one key head for all: stride 0
+    o, b = reference_many(q, pk, pv, k1, v1, cu_q, cu_k, True)
+    close(cache.attention(e, 1, q, k1, v1, dev(cu_q), dev(cu_k)), o, b)
+    q1 = q[:, :1].expand(-1, 6, -1)
+    o, b = reference_many(q1, pk, pv, k, v, cu_q, cu_k, True)
+    close(cache.attention(e, 1, q1, k, v, dev(cu_q), dev(cu_k)), o, b)
+    own = q.clone()                                              # the output in q's place
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    cache.attention(e, 1, own, k, v, dev(cu_q), dev(cu_k), out=own)
+    close(own, o, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_both_forms_of_the_probabilities(pc, dtype):
+    """few rows keep the probabilities in two parts: the error is the output's rounding alone; many rows keep one part"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, 8, 2, 128, 500, [300, 212, 88])
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))                   # 4800 rows
+    close(out, o, b)
+    few = cache.attention(e, 1, q[:500], k[:512], v[:512], dev([0, 300, 500]), dev([0, 300, 512]))   # 4000 rows
+    o2, b2 = reference_many(q[:500], pk, pv, k[:512], v[:512], [0, 300, 500], [0, 300, 512], True)
+    h = torch.finfo(dtype).eps / 2                               # (and h^2 b of what the second part leaves)
+    assert ((few.double() - o2).abs() <= h * o2.abs() * (1 + h) + (h * h + 4e-4) * b2 + 1e-7).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # streams, graphs, refusals
 # ---------------------------------------------------------------------------------------------------------------
