@@ -409,7 +409,8 @@ class SentenceTransformer:
         `prompt`: the string that `encode(prompt=...)` puts in front of every text, or a list of token ids; `prompt_name`: one of
         `prompts` (None: the default prompt).  Causal models only -- in a bidirectional one (stella, gte-Qwen2) the prompt's
         hidden states depend on the text behind it.  Returns how many tokens are held; the embeddings are the same to bf16
-        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before.  A prompt that begins as one
+        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before (so is a single query of at most 32
+        tokens with its prompt: that is faster).  A prompt that begins as one
         that is cached shares its pages.  `load_weights` drops all of them."""
         import torch
         if not self.config.get("causal"):
@@ -490,6 +491,12 @@ class SentenceTransformer:
             behind = [self._behind(t) for t in token_lists]
             for i, (_, handle) in enumerate(behind):
                 by.setdefault(handle, []).append(i)
+            for handle, members in list(by.items()):
+                # one query of at most 32 tokens with its prompt: the query-time path, with the attention inside its O projection, is
+                # faster over all of them (1.09 ms) than over the query's own behind the cached prompt (1.21 ms)
+                if handle is not None and len(members) == 1 and len(token_lists[members[0]]) <= 32:
+                    behind[members[0]] = (0, None)
+                    by.setdefault(None, []).extend(by.pop(handle))
             token_lists = [t[k:] for t, (k, _) in zip(token_lists, behind)]
             groups = list(by.items())
         for handle, members in groups:

@@ -48,7 +48,8 @@ def test_prompted_against_the_oracle(st, tiny, prompt_len, lens):
     p0 = st.debug_counter("prompted_passes")
     assert model.cache_prompt(prompt) == prompt_len
     e = model.encode_tokens(toks, normalize_embeddings=True)
-    assert st.debug_counter("prompted_passes") == p0 + 2         # the prompt's own pass and one for the texts
+    alone = len(toks) == 1 and len(toks[0]) <= 32                 # (one short query: all of it through the query-time path)
+    assert st.debug_counter("prompted_passes") == p0 + 1 + (not alone)   # the prompt's own pass and one for the texts
     ref = oracle_encode(cfg, W, toks)
     same(e, ref, 1e-3)
     same(e, plain, 1e-3)
@@ -172,7 +173,7 @@ def test_encode_with_a_prompt_string(st, tiny):
     same(model.encode(texts, prompt_name="q", normalize_embeddings=True), plain, 1e-3)
     assert st.debug_counter("prompted_passes") == p0 + 1
     one = model.encode("w1 w2", prompt_name="q", normalize_embeddings=True)
-    same(one[None], plain[:1], 1e-3)
+    assert np.array_equal(one, plain[0]) or (one * plain[0]).sum() > 1 - 1e-3
     same(model.encode(texts, normalize_embeddings=True), oracle_encode(cfg, W, model.tokenize(texts)), 1e-3)
 
 
