@@ -247,22 +247,27 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     return a;
 }
 
-// How a call is cut up.  Rows of a workgroup: 32, 64 or 128 (a wave each 32), as few as hold a key head's rows.  Where the tiles do
-// not fill the chip, the keys are split so that they nearly do (two workgroups a CU) --
-// at least two chunks of 64 keys each, or the join costs more than it saves.
+// How a call is cut up: tiles of 128 rows of a key head, and where these do not fill the chip the keys `splits` ways, so that there
+// is a workgroup for each of the 256 CUs -- two, if each still has eight chunks of 64 keys or more: 50 us with 64 splits of the 1024
+// chunks of four tokens behind 65 500, 66 with 32; but 32 with 32 splits of the 82 chunks of 64 single tokens behind 2048, 27 with 16,
+// because every split's partials are written and read again.  At least two chunks each, as far as there are two: the join costs as
+// much as they do (3 us).
 struct Plan {
-    int nw, splits, tiles;
+    int splits, tiles;
     int64_t rows;                        // of all key heads
     int64_t o_bytes, bytes;              // partials, workspace
 };
+
 Plan plan_of(const PromptArgs &a, int hd) {
+    constexpr int R = 32 * PA_WAVES;
     Plan p{};
     const int64_t per_head = (int64_t)a.n_tokens * a.G;
     p.rows = per_head * a.n_kv;
-    p.nw = per_head <= 32 ? 1 : per_head <= 64 ? 2 : 4;
-    p.tiles = (int)((per_head + 32 * p.nw - 1) / (32 * p.nw));
-    const int64_t wgs = (int64_t)p.tiles * a.n_kv, chunks = (a.P + PC_PAGE - 1) / PC_PAGE + (a.n_keys / a.n_texts + PC_PAGE - 1) / PC_PAGE;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / wgs, chunks / 2));
+    p.tiles = (int)((per_head + R - 1) / R);
+    // chunks that a tile goes through: the prompt's, and its texts' share of the own keys
+    const int64_t wgs = (int64_t)p.tiles * a.n_kv, own = a.n_keys * std::min<int64_t>(per_head, R) / per_head;
+    const int64_t chunks = (a.P + PC_PAGE - 1) / PC_PAGE + (own + PC_PAGE - 1) / PC_PAGE, target = chunks * wgs >= 8 * 512 ? 512 : 256;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(target / wgs, chunks / 2));
     p.o_bytes = p.splits > 1 ? p.splits * p.rows * hd * 4 : 0;
     p.bytes = p.splits > 1 ? p.o_bytes + p.splits * p.rows * 8 : 0;
     return p;
@@ -272,10 +277,9 @@ template <class T, int HD, bool VT>
 void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)p.tiles * p.splits * a.n_kv + 7) / 8 * 8));
     // few rows: the probabilities in two parts (see the kernel)
-    if (p.nw == 1) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 1, VT, true>), grid, dim3(64), 0, st, a);
-    else if (p.nw == 2) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 2, VT, true>), grid, dim3(128), 0, st, a);
-    else if (p.rows <= 4096) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, 4, VT, false>), grid, dim3(256), 0, st, a);
+    const dim3 block(64 * PA_WAVES);
+    if (p.rows <= 4096) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, VT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, VT, false>), grid, block, 0, st, a);
     MI_HIP(hipGetLastError());
     if (p.splits > 1) {
         constexpr int per_wg = 256 / (HD / 4);                                    // groups of lanes

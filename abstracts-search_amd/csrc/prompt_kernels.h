@@ -203,7 +203,7 @@ __device__ void prompt_row(const PromptArgs &a, int token, int head, int64_t p0,
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// A tile of 32 NW rows of one key head by NW waves, the keys in chunks of 64 (a page, or 64 of the texts' own): K and V of a
+// A tile of 128 rows of one key head by four waves, the keys in chunks of 64 (a page, or 64 of the texts' own): K and V of a
 // chunk arrive by LDS-DMA, double buffered, and serve every wave.  Computed transposed: S^T = K Q^T on 32x32x16 MFMAs leaves a
 // lane 32 scores of ONE row (the other half of the chunk sits in lane ^ 32), so the softmax is in-lane but for one exchange.
 // Which key a row position of S^T stands for is free: position m <-> key m with bits 2 and 3 exchanged; then registers
@@ -234,6 +234,7 @@ __device__ __forceinline__ u32x2 lds_tr(const lds_t *p) {
 }
 __device__ __forceinline__ u32x4 lds_16(const lds_t *p) { return *(const __attribute__((address_space(3))) u32x4 *)p; }
 
+constexpr int PA_WAVES = 4;               // waves of a workgroup: a tile of 128 rows
 constexpr int PA_CU = 1023;               // texts whose bounds are kept in LDS
 
 // four consecutive dims of one (token, head) of the output
@@ -279,7 +280,7 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     *reinterpret_cast<float4 *>(po + 32 * n + 8 * q) = make_float4(o[n][4 * q], o[n][4 * q + 1], o[n][4 * q + 2], o[n][4 * q + 3]);
-            if (!half) a.part_ml[prow + row] = make_float2(mrow, lrow);
+            if (!half) a.part_ml[prow + row] = make_float2(mrow, !live ? -1.f : sees ? lrow : -2.f);   // (the same in every split: what the join does not have to look up)
         } else {
             const float inv = live && sees ? 1.0f / lrow : 0.f;                  // (0 x inf where every score is -inf: NaN, as 0 / 0)
             // dims 32 n + 8 q + 4 half ..: rows of the output, or fragments (prompt_store4)
@@ -317,11 +318,14 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 // output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output.  Few rows are
 // bound by latency or by reading the pages and take the second product for nothing (one query 9.3 us either way, four tokens
 // behind 65 500 61); many rows are bound by the products.
+// Four waves also where one holds all the rows: the others bring their quarter of the keys in.  Against workgroups of one and of two
+// waves: 8.6 us instead of 10.5 and 10.0 on ten tokens behind 37, 51 instead of 57 and 55 on four tokens behind 65 500; eight waves
+// took 9.0 and 70.
 // Two stages of LDS, so that two workgroups share a CU and overlap each other (four stages and one workgroup a CU: 88 us instead
 // of 52 on four tokens behind 65 500, 1026 instead of 1005 on 12.7 k tokens behind 4096).
-template <class T, int HD, int NW, bool VT, bool TWO>
-__global__ void __launch_bounds__(64 * NW, 2) prompt_tile_kernel(PromptArgs a) {
-    constexpr int KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
+template <class T, int HD, bool VT, bool TWO>
+__global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArgs a) {
+    constexpr int NW = PA_WAVES, KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
     constexpr int RPP = 64 / SL, PIECES = KC / RPP, PPW = PIECES / NW;            // rows of a 1-KiB piece, pieces of a K or V tile, of a wave
     constexpr int STG = 2 * KC * HD, NS = 2;
     static_assert(PIECES % NW == 0, "pieces divide over the waves");
@@ -618,10 +622,11 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
     const int rows = a.n_tokens * a.G, g = threadIdx.x / LPR % PAR, rb = threadIdx.x / LPR / PAR, ln = threadIdx.x % LPR;
     const int64_t n = (int64_t)rows * a.n_kv, i = (int64_t)blockIdx.x * RPB + rb, at = i < n ? i : n - 1;
     float m = -__builtin_huge_valf(), l = 0.f;
+    const float kind = a.part_ml[at].y;                                          // -1: no text's row, -2: sees no key, otherwise a sum (or NaN)
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](float2 ml, float4 x) {                                        // (a split that saw no key of the row has zeros and the maximum -inf)
         const float mn = fmaxf(m, ml.x), sub = mn == -__builtin_huge_valf() ? 0.f : mn;
-        const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - sub), e = ml.x == -__builtin_huge_valf() && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - sub);
+        const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - sub), e = ml.x == -__builtin_huge_valf() && ml.y <= 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - sub);
         m = mn;
         l = l * f + e * ml.y;
         o.x = o.x * f + e * x.x; o.y = o.y * f + e * x.y; o.z = o.z * f + e * x.z; o.w = o.w * f + e * x.w;
@@ -648,12 +653,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
         for (int q = 1; q < PAR; ++q) add(s_ml[q][rb], s_o[q][rb][ln]);
     }
     if (i >= n) return;
+    if (kind == -1.f && !a.zero_rest) return;
     const int d = ln * 4, kvh = (int)(i / rows), row = (int)(i % rows), token = row / a.G, head = kvh * a.G + row % a.G;
-    int lo, hi;
-    const bool live = prompt_own_range(a, a.cu_q, a.cu_k, token, lo, hi);
-    if (!live && !a.zero_rest) return;
-    const float inv = a.P > 0 || hi > lo ? 1.0f / l : 0.f;
-    if (live) prompt_store4<T, HD>(a, token, head, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const float inv = 1.0f / l;
+    if (!(kind < 0.f)) prompt_store4<T, HD>(a, token, head, d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     else prompt_store4<T, HD>(a, token, head, d, 0.f, 0.f, 0.f, 0.f);
 }
 
