@@ -56,7 +56,7 @@ struct TBf16 {
     __device__ static unsigned pack(float lo, float hi) { return pack2(lo, hi); }
     __device__ static unsigned scaled(unsigned two, float f) { return pack(up((unsigned short)(two & 0xffffu)) * f, up((unsigned short)(two >> 16)) * f); }
     __device__ static unsigned short down(float v) { return (unsigned short)(pack2(v, v) & 0xffffu); }
-    // probabilities are rounded to the values' type for the product with V (relative error 2^-9 each, the denominator sums the
+    // probabilities are rounded to the values' type for the product with V (a relative error of up to 2^-8 each, the denominator sums the
     // f32 values); bf16 has f32's exponents
     static constexpr float shift = 0.f;
 };
@@ -268,9 +268,9 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
     for (int n = 0; n < NDT; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(o[n][r], 0.f, zero);
-    uint64_t redo = __builtin_amdgcn_ballot_w64(zero != 0.f && live);
+    const bool sees = live && (a.P > 0 || hi > lo);
+    uint64_t redo = __builtin_amdgcn_ballot_w64(zero != 0.f && sees);
     redo = (redo | redo >> 32) & 0xffffffffu;
-    const bool sees = a.P > 0 || hi > lo;
     const int64_t prow = ((int64_t)split * a.n_kv + kvh) * rows;                 // this split's partials of the key head
     if (row < rows && !(redo >> li & 1) && (live || a.zero_rest || a.splits > 1)) {
         if (a.splits > 1) {
@@ -282,7 +282,7 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
                     *reinterpret_cast<float4 *>(po + 32 * n + 8 * q) = make_float4(o[n][4 * q], o[n][4 * q + 1], o[n][4 * q + 2], o[n][4 * q + 3]);
             if (!half) a.part_ml[prow + row] = make_float2(mrow, !live ? -1.f : sees ? lrow : -2.f);   // (the same in every split: what the join does not have to look up)
         } else {
-            const float inv = live && sees ? 1.0f / lrow : 0.f;                  // (0 x inf where every score is -inf: NaN, as 0 / 0)
+            const float inv = 1.0f / lrow;                  // (0 x inf where every score is -inf: NaN, as 0 / 0)
             // dims 32 n + 8 q + 4 half ..: rows of the output, or fragments (prompt_store4)
             bf16_t *po = (a.frag ? a.frag + (((int64_t)head * (HD / 32) * a.frag_mt + (token >> 4)) * 64 + (token & 15)) * 8 : a.out + token * a.o_token + head * a.o_head) + 4 * half;
             const int sn = a.frag ? a.frag_mt * 512 : 32, sq = a.frag ? 128 : 8;
@@ -291,7 +291,7 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint2 v = make_uint2(T::pack(o[n][4 * q] * inv, o[n][4 * q + 1] * inv), T::pack(o[n][4 * q + 2] * inv, o[n][4 * q + 3] * inv));
-                    if (!live) v = make_uint2(0u, 0u);
+                    if (!sees) v = make_uint2(0u, 0u);
                     *reinterpret_cast<uint2 *>(po + q * sq) = v;
                 }
         }

@@ -467,6 +467,37 @@ def test_nothing_to_see_and_broadcast_operands(pc):
     close(own, o, b)
 
 
+@pytest.mark.parametrize("prompt,first", [(0, 0), (1000, 0), (0, 9)])
+def test_split_keys_and_rows_without_any(pc, prompt, first):
+    """few rows and many keys of their own: the keys are split, and the join has to know which rows see nothing, belong to no text,
+    or were done again (what is masked holds no numbers)"""
+    lens, past = [1] * 9 + [0, 30, 1] + [1] * 9, [300, 0, 7, 64, 1, 130, 0, 500, 2, 0, -20, -1] + [90] * 9
+    lens, past, at = lens[first:], past[first:], 10 - first   # (from the tenth on: too few keys to split)
+    if first:
+        lens, past = lens[:3], past[:3]
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 8, 2, 128, prompt, lens, past)
+    assert first or cu_k[-1] > 1000
+    # text `at`: 30 queries on 10 keys, the first 20 of which see none of them; the one behind it: no key at all
+    v[cu_k[at] + 5:cu_k[at + 1]] = math.nan                       # .. and the rows before the 26th see none of these
+    tail = 3                                                  # rows of no text
+    qq = torch.cat([q, q[:tail]])
+    out = torch.full_like(qq, 7.0)
+    cache.attention(e, 1, qq, k, v, dev(cu_q), dev(cu_k), out=out)
+    assert (out[-tail:] == 7.0).all()
+    fresh = cache.attention(e, 1, qq, k, v, dev(cu_q), dev(cu_k))
+    assert (fresh[-tail:] == 0).all() and torch.equal(fresh[:-tail].isnan(), out[:-tail].isnan())
+    assert torch.equal(fresh[:-tail].nan_to_num(), out[:-tail].nan_to_num())
+    r0, r1 = cu_q[at] + 25, cu_q[at + 1]
+    assert out[r0:r1].isnan().all()
+    if not prompt:
+        assert (out[cu_q[at]:cu_q[at] + 20] == 0).all() and (out[cu_q[at + 1]:cu_q[at + 2]] == 0).all()
+    v[cu_k[at] + 5:cu_k[at + 1]] = 0
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    keep = torch.ones(q.shape[0], dtype=torch.bool, device="cuda")
+    keep[r0:r1] = False
+    close(out[:-tail][keep], o[keep], b[keep])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_both_forms_of_the_probabilities(pc, dtype):
     """few rows keep the probabilities in two parts: the error is the output's rounding alone; many rows keep one part"""
