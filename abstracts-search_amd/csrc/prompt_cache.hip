@@ -18,6 +18,8 @@ namespace {
 hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 // stands for "whatever work used it is done": a page or an entry's place may be used on any stream
 void *const ANY = reinterpret_cast<void *>(~uintptr_t(0));
+// .. and for work of several streams: equal to none, so that whoever takes the page waits for the device
+void *const SEVERAL = reinterpret_cast<void *>(~uintptr_t(1));
 
 bool capturing(void *stream) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -64,7 +66,7 @@ struct mi_prompt_cache {
     DevBuf own, tables;
     std::mutex mu;
     std::vector<int32_t> ref;            // entries that hold the page
-    std::vector<void *> tag;             // of a free page: the stream whose work may still read it
+    std::vector<void *> tag;             // the stream on which entries gave the page up: their work may still read it
     PageSet free_pages;
     std::vector<Entry> entries;
 
@@ -76,7 +78,7 @@ struct mi_prompt_cache {
 
     void wait_all() {                    // everything issued so far is done: whatever is free is free for every stream
         MI_HIP(hipDeviceSynchronize());
-        free_pages.each([&](int32_t p) { tag[p] = ANY; return true; });
+        std::fill(tag.begin(), tag.end(), ANY);
         for (Entry &e : entries)
             if (!e.live) e.slot_tag = ANY;
     }
@@ -90,7 +92,11 @@ struct mi_prompt_cache {
             if (tag[p] != ANY && tag[p] != stream) { wait_all(); break; }
         return got;
     }
-    void take(int32_t p) { free_pages.erase(p); ref[p] = 1; }
+    void take(int32_t p) { free_pages.erase(p); ref[p] = 1; tag[p] = ANY; }
+    void drop(int32_t p, void *stream) {
+        if (stream != ANY) tag[p] = tag[p] == ANY || tag[p] == stream ? stream : SEVERAL;
+        if (--ref[p] == 0) free_pages.insert(p);
+    }
     std::vector<int32_t> pick_entries(int n, void *stream) {
         std::vector<int32_t> got;
         for (int32_t e = 0; e < (int32_t)entries.size() && (int)got.size() < n; ++e)
@@ -527,8 +533,7 @@ int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *list, voi
         void *const tag = wait ? ANY : stream;
         for (int32_t i = 0; i < n; ++i) {
             Entry &e = c->entries[list[i]];
-            for (int32_t p : e.pages)
-                if (--c->ref[p] == 0) { c->free_pages.insert(p); c->tag[p] = tag; }
+            for (int32_t p : e.pages) c->drop(p, tag);
             e.live = false;
             e.len = 0;
             e.pages.clear();
@@ -555,7 +560,8 @@ int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
         if (src.empty()) return;
         bool cross = false;
         for (const Entry &e : c->entries) cross = cross || (e.live && (e.foreign || e.home != stream));
-        for (int32_t p : dst) cross = cross || (c->tag[p] != ANY && c->tag[p] != stream);
+        for (const std::vector<int32_t> *pages : {&dst, &src})
+            for (int32_t p : *pages) cross = cross || (c->tag[p] != ANY && c->tag[p] != stream);
         if (cross) c->wait_all();
         c->copy_pages(c->pages, c->pages, src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream));
         c->remap(src.data(), dst.data(), (int)src.size(), as_stream(stream));
@@ -567,6 +573,7 @@ int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
             c->ref[src[j]] = 0;
             c->free_pages.erase(dst[j]);
             c->free_pages.insert(src[j]);
+            c->tag[dst[j]] = ANY;
             c->tag[src[j]] = stream;
         }
         for (Entry &e : c->entries)

@@ -564,6 +564,66 @@ def test_another_stream_and_freed_pages(pc):
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_pages_given_up_on_several_streams(pc):
+    """two forks on streams of their own share a page: whoever gives it up first may still read it when the other's stream takes
+    the page for something else, so that stream waits"""
+    cache = pc.PromptCache(1, 1, 64, 4, max_entries=6)
+    home, s1, s2 = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    kv = torch.randn(1, 64, 1, 64, device="cuda", dtype=BF)
+    parent = cache.new()
+    cache.extend(parent, kv, kv)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        a = cache.fork(parent)[0]
+    with torch.cuda.stream(s2):
+        b = cache.fork(parent)[0]
+    assert cache.table(a) == cache.table(b) == [0]
+    cache.free(parent)
+    q = torch.randn(1, 2, 64, device="cuda", dtype=BF)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        torch.cuda._sleep(20_000_000)                         # ~10 ms of s1 before it reads
+        out = cache.attention(a, 0, q)
+        cache.free(a)
+        read = torch.cuda.Event()
+        read.record()
+    with torch.cuda.stream(s2):
+        cache.free(b)
+        c = cache.new()
+        cache.extend(c, kv * 0, kv * 0)
+        assert cache.table(c) == [0] and read.query()         # the host came back behind s1's reading
+    torch.cuda.synchronize()
+    w = torch.softmax(kv[0, :, 0].double() @ q[0].double().t() / 8, 0)
+    o, m = w.t() @ kv[0, :, 0].double(), w.t() @ kv[0, :, 0].double().abs()
+    close(out, o[None], m[None])
+    # the same with a page that is moved: what a's stream reads stays until it is done
+    cache.free(c)
+    low = cache.new()
+    cache.extend(low, kv, kv)
+    with torch.cuda.stream(s2):
+        up = cache.new()
+        cache.extend(up, kv, kv)
+        assert cache.table(up) == [1]
+        with torch.cuda.stream(s1):
+            x = cache.fork(up)[0]
+            y = cache.fork(up)[0]
+        cache.free(up)
+        cache.free(x)                                         # (another stream's: waits)
+    with torch.cuda.stream(s1):
+        z = cache.fork(y)[0]
+        cache.free(y)
+        torch.cuda._sleep(20_000_000)
+        out = cache.attention(z, 0, q)
+    cache.free(low)
+    assert cache.compact() == 1 and cache.table(z) == [0]
+    with torch.cuda.stream(s1):
+        again = cache.attention(z, 0, q)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+    close(out, o[None], m[None])
+    assert home == torch.cuda.current_stream()
+
+
 def test_refusals(pc):
     cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [5])
     bad = [
