@@ -712,15 +712,11 @@ struct mi_encoder {
     int few_gen = -1;        // ... for this generation of the knobs (g_knob_gen)
     bool few_gu8 = false;    // ... and the gate/up pieces are few_gu8_kernel's (8 gate + 8 up rows per piece)
     bool roped_ok = false;   // the rotary-pair-interleaved QKV copies are current
-    // profiling: the GEMM launches of the most recent encode (arguments as launched), replayed back to back between two
-    // HIP events by mi_encoder_profile_read -- like the index library's scan replay; per-launch event pairs measured
-    // 3-4 % short of rocprofv3's per-kernel durations in the same run
     // cached prompts (causal models): their keys and values live in one pool of pages, the sum of their final hidden states beside
     // them.  A pass holds a reference, so that a prompt dropped meanwhile goes when the pass has been issued.
     struct Prompt {
         mi_prompt_cache *cache = nullptr;
         int32_t entry = -1;
-        void *stream = nullptr;              // it was made on
         int device = 0;
         std::vector<int32_t> ids;
         DevBuf sum;                          // f32 [hidden]: the tokens' final-norm hidden states (bf16 values, as the pooling sees them)
@@ -729,7 +725,7 @@ struct mi_encoder {
             int prev = 0;
             (void)hipGetDevice(&prev);
             (void)hipSetDevice(device);
-            (void)mi_prompt_cache_free(cache, 1, &entry, stream);
+            (void)mi_prompt_cache_free(cache, 1, &entry, nullptr);   // (the stream it was made on may be gone)
             sum.release();
             (void)hipSetDevice(prev);
         }
@@ -743,6 +739,9 @@ struct mi_encoder {
         prompts.clear();
         if (prompt_cache) (void)mi_prompt_cache_destroy(prompt_cache);
     }
+    // profiling: the GEMM launches of the most recent encode (arguments as launched), replayed back to back between two
+    // HIP events by mi_encoder_profile_read -- like the index library's scan replay; per-launch event pairs measured
+    // 3-4 % short of rocprofv3's per-kernel durations in the same run
     bool prof = false;
     struct Launch { int epi; GemmArgs g; };
     std::vector<Launch> prof_launches;
@@ -1762,7 +1761,6 @@ int mi_encoder_cache_prompt(mi_encoder *h, int n, const int32_t *ids, int32_t *p
         }
         auto p = std::make_shared<mi_encoder::Prompt>();
         p->cache = h->prompt_cache;
-        p->stream = stream;
         p->device = h->device;
         p->ids.assign(ids, ids + n);
         if (base ? mi_prompt_cache_fork(h->prompt_cache, base->entry, 1, &p->entry, nullptr, stream) : mi_prompt_cache_new(h->prompt_cache, stream, &p->entry))

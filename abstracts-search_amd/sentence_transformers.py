@@ -409,9 +409,9 @@ class SentenceTransformer:
         `prompt`: the string that `encode(prompt=...)` puts in front of every text, or a list of token ids; `prompt_name`: one of
         `prompts` (None: the default prompt).  Causal models only -- in a bidirectional one (stella, gte-Qwen2) the prompt's
         hidden states depend on the text behind it.  Returns how many tokens are held; the embeddings are the same to bf16
-        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before (so is a single query of at most 32
-        tokens with its prompt: that is faster).  A prompt that begins as one
-        that is cached shares its pages.  `load_weights` drops all of them."""
+        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before, and so is a single query of at
+        most 32 tokens with its prompt (that is faster).  A prompt that begins as one that is cached shares its pages.
+        `load_weights` drops all of them."""
         import torch
         if not self.config.get("causal"):
             raise ValueError("cache_prompt needs a causal model: in a bidirectional one the prompt's hidden states depend on the text behind it")
