@@ -352,7 +352,9 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
 
     auto swz = [](int key) { return SL == 16 ? (key & 3) << 2 | ((key >> 2) & 3) : ((key >> 1) & 1) << 2 | ((key >> 3) & 1) << 1 | (key & 1); };
     const bf16_t *const head_pages = a.pages + (int64_t)kvh * 2 * KC * HD;
-    int next_page = np > 0 ? __builtin_amdgcn_readfirstlane(a.table[p0]) : 0;                                   // (read a chunk ahead: its latency is not the request's)
+    // the numbers of 64 pages, one in each lane (a number fetched for each chunk would be waited for with everything in flight)
+    auto pages_from = [&](int i) { return a.table[min(p0 + i + lane, nP - 1)]; };
+    int numbers = np > 0 ? pages_from(0) : 0;
     auto issue = [&](int i) {
         lds_t *Ks = smem + (i % NS) * STG, *Vs = Ks + KC * HD;
         // the base of a chunk is uniform, a lane adds 32 bits (the host bounds the strides)
@@ -362,9 +364,12 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
         const bool own = i >= np;
         const int b = base_of(i);
         if (!own) {
-            kb = head_pages + next_page * a.page_stride;
+            kb = head_pages + __builtin_amdgcn_readlane(numbers, i & 63) * a.page_stride;
             vb = kb + KC * HD;
-            next_page = __builtin_amdgcn_readfirstlane(a.table[min(p0 + i + 1, nP - 1)]);
+            if ((i & 63) == 63) {
+                numbers = pages_from(i + 1);
+                asm volatile("" : "+v"(numbers));                                // (waited for here)
+            }
             last = min(last, a.P - 1 - b);
         } else {
             kb = a.k + b * a.k_token + kvh * a.k_head;
@@ -434,6 +439,7 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
             if (i <= a.n_texts) { s_cu[0][i] = b_q[e]; s_cu[1][i] = b_k[e]; }
         }
     }
+    pin_q();                                                                     // (came in beside the bounds; the compiler's wait for them behind the first chunks would be one for these too)
     const int early = min(np, NS);
     for (int i = 0; i < early; ++i) issue(i);
     if (in_lds) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -462,7 +468,6 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
     o0 = a.splits > 1 ? (int)((int64_t)nO * split / a.splits) : 0;
     const int n = np + (a.splits > 1 ? (int)((int64_t)nO * (split + 1) / a.splits) : nO) - o0;
     for (int i = early; i < min(n, NS); ++i) issue(i);
-    pin_q();
     f32x16 o[NDT];
 #pragma unroll
     for (int d = 0; d < NDT; ++d) o[d] = (f32x16)(0.f);
