@@ -282,9 +282,9 @@ Plan plan_of(const PromptArgs &a, int hd) {
 template <class T, int HD, bool VT>
 void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)p.tiles * p.splits * a.n_kv + 7) / 8 * 8));
-    // few rows: the probabilities in two parts (see the kernel)
+    // few rows of a key head: the probabilities in two parts (see the kernel)
     const dim3 block(64 * PA_WAVES);
-    if (p.rows <= 4096) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, VT, true>), grid, block, 0, st, a);
+    if (p.tiles <= 2) hipLaunchKernelGGL((prompt_tile_kernel<T, HD, VT, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((prompt_tile_kernel<T, HD, VT, false>), grid, block, 0, st, a);
     MI_HIP(hipGetLastError());
     if (p.splits > 1) {

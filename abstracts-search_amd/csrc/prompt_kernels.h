@@ -315,14 +315,23 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 }
 
 // TWO: the probabilities enter the product with V in two parts (what the type holds of them, and of the rest), which leaves the
-// output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output.  Few rows are
-// bound by latency or by reading the pages and take the second product for nothing (one query 9.3 us either way, four tokens
-// behind 65 500 61); many rows are bound by the products.
+// output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output (error against 64
+// bits 0.0024 instead of 0.0017 in bf16).  Taken where a key head's rows are two tiles at most, which latency and the reading of the
+// pages bound: 8.6 us instead of 8.0 on ten tokens behind 37, 26.4 instead of 24.8 on 64 single tokens of 32 heads behind 2048.  More
+// rows are bound by the products: 66 instead of 53 on 40 tokens of 64 heads behind 20 000, 1347 instead of 1018 on 12.7 k behind 4096.
 // Four waves also where one holds all the rows: the others bring their quarter of the keys in.  Against workgroups of one and of two
-// waves: 8.6 us instead of 10.5 and 10.0 on ten tokens behind 37, 51 instead of 57 and 55 on four tokens behind 65 500; eight waves
+// waves: 8.6 us instead of 10.5 and 10.0 on ten tokens behind 37, 50 instead of 57 and 55 on four tokens behind 65 500; eight waves
 // took 9.0 and 70.
-// Two stages of LDS, so that two workgroups share a CU and overlap each other (four stages and one workgroup a CU: 88 us instead
-// of 52 on four tokens behind 65 500, 1026 instead of 1005 on 12.7 k tokens behind 4096).
+// Two stages of LDS, so that two workgroups share a CU and overlap each other: four stages and one workgroup a CU took 1.7 times as
+// long on four tokens behind 65 500 and 2 % longer on 12.7 k behind 4096, and four stages beside two workgroups (head dim 64) 4 %
+// longer on 4 k tokens of 16 heads behind 1000.
+// What bounds it, and what it takes with its join, launches included:
+//   few rows, short prompt    latency: launch, arguments, bounds and Q, first page, two chunks, store; 8.9 us (10 tokens behind 37)
+//   few rows, long prompt     reading the pages: 57 us for the 269 MB of 65 500 tokens (the kernel 47: 5.7 TB/s), 25.6 us for 64
+//                             single tokens with pasts (35 MB) behind 2048: 18 + 7.5 for the partials of 16 splits
+//   many rows                 matrix and vector work in turn at the clock that the power limit leaves (1.8 GHz): 990 us for 12.7 k
+//                             tokens of 32 heads of 128 behind 4096, 920 TFLOP/s (products alone, without the exponentials, 652 us);
+//                             head dim 64: the exponentials, 40 us for 4 k tokens of 16 heads behind 1000
 template <class T, int HD, bool VT, bool TWO>
 __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArgs a) {
     constexpr int NW = PA_WAVES, KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
@@ -618,7 +627,8 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
 
 // the splits' partials of a row -> the output: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  HD / 4 lanes hold four dims each; PAR
 // such groups take every PAR-th split of a row (8 where there are more than 8 splits: one group would go through them as one chain
-// of loads, 34 us at 64 splits) and meet in LDS, always in the same order.
+// of loads, 34 us at 64 splits) and meet in LDS, always in the same order.  Bound by latency (4.2 us for 128 rows x 64 splits of
+// 128 dims) and by the L2s' 17 MB of partials (7.3 us for 2048 rows x 16 splits: 2.3 TB/s).
 template <class T, int HD, int PAR>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR / PAR;                           // lanes of a group, rows of a workgroup
@@ -668,7 +678,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // Pages
 // ---------------------------------------------------------------------------------------------------------------------
-// page numbers into an entry's table (they travel as kernel arguments: stream order is all that a later reader needs)
+// What moves keys and values is bound by HBM where it moves much and by the launch (3 - 4 us) where it does not; a thread moves 16
+// bytes, neighbours neighbouring ones on both sides.
+
+// page numbers into an entry's table (they travel as kernel arguments: stream order is all that a later reader needs); 1.4 us
 struct PcTableArgs {
     int32_t *dst;
     int n;
@@ -678,7 +691,8 @@ __global__ void __launch_bounds__(256) pc_table_kernel(PcTableArgs a) {
     for (int i = threadIdx.x; i < a.n; i += 256) a.dst[i] = a.val[i];
 }
 
-// keys and values of n tokens into the pages of an entry: a thread per (layer, token, key head, 8 dims) and K / V.
+// keys and values of n tokens into the pages of an entry: a thread per (layer, token, key head, 8 dims) and K / V.  4000 tokens of 28
+// layers (229 MB read and written): 36 us, 6.4 TB/s; 37 tokens: 3.2 us.
 // k_inter: the source's dims are interleaved by rotary pair (2 f + h = pair f, half h); v_dim != 1: the source is V^T, elements
 // v_dim apart.  Both only where the encoder stores a prompt, once.
 struct PcWriteArgs {
@@ -722,7 +736,9 @@ __global__ void __launch_bounds__(256) pc_write_kernel(PcWriteArgs a) {
     for (int j = 0; j < 8; ++j) dst[j] = src[j * st];
 }
 
-// the first `rows` rows of every (layer, key head, K / V) of page src[j] -> page dst[j].  grid (blocks, jobs)
+// the first `rows` rows of every (layer, key head, K / V) of page src[j] -> page dst[j].  grid (blocks, jobs): a thread takes four
+// words, so that a launch of a few pages fills the chip too.  200 pages of 28 layers (734 MB read and written): 128 us, 5.7 TB/s; 200
+// copies of 40 rows of one page: 35 us; four: 4.0.
 struct PcCopyArgs {
     const bf16_t *from;
     bf16_t *to;
@@ -767,7 +783,8 @@ __global__ void __launch_bounds__(256) pc_fork_kernel(PcForkArgs a) {
     for (int i = threadIdx.x; i < a.shared; i += 256) t[i] = p[i];
 }
 
-// page numbers src[j] -> dst[j] in every table (src ascending; words behind an entry's length may change too, nothing reads them)
+// page numbers src[j] -> dst[j] in every table (src ascending; words behind an entry's length may change too, nothing reads them);
+// a word each thread and a search in LDS: 4.6 us for 200 moves in 4 tables of 400 pages, latency
 struct PcRemapArgs {
     int32_t *tables;
     int64_t words;
