@@ -318,18 +318,18 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 // output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output (error against 64
 // bits 0.0024 instead of 0.0017 in bf16).  Taken where a key head's rows are two tiles at most, which latency and the reading of the
 // pages bound: 8.6 us instead of 8.0 on ten tokens behind 37, 26.4 instead of 24.8 on 64 single tokens of 32 heads behind 2048.  More
-// rows are bound by the products: 66 instead of 53 on 40 tokens of 64 heads behind 20 000, 1347 instead of 1018 on 12.7 k behind 4096.
+// rows are bound by the products: 66 instead of 53 on 40 tokens of 64 heads behind 20 000, 1347 instead of 1018 on 13.1 k behind 4096.
 // Four waves also where one holds all the rows: the others bring their quarter of the keys in.  Against workgroups of one and of two
 // waves: 8.6 us instead of 10.5 and 10.0 on ten tokens behind 37, 50 instead of 57 and 55 on four tokens behind 65 500; eight waves
 // took 9.0 and 70.
 // Two stages of LDS, so that two workgroups share a CU and overlap each other: four stages and one workgroup a CU took 1.7 times as
-// long on four tokens behind 65 500 and 2 % longer on 12.7 k behind 4096, and four stages beside two workgroups (head dim 64) 4 %
+// long on four tokens behind 65 500 and 2 % longer on 13.1 k behind 4096, and four stages beside two workgroups (head dim 64) 4 %
 // longer on 4 k tokens of 16 heads behind 1000.
 // What bounds it, and what it takes with its join, launches included:
 //   few rows, short prompt    latency: launch, arguments, bounds and Q, first page, two chunks, store; 8.9 us (10 tokens behind 37)
 //   few rows, long prompt     reading the pages: 57 us for the 269 MB of 65 500 tokens (the kernel 47: 5.7 TB/s), 25.6 us for 64
 //                             single tokens with pasts (35 MB) behind 2048: 18 + 7.5 for the partials of 16 splits
-//   many rows                 matrix and vector work in turn at the clock that the power limit leaves (1.8 GHz): 990 us for 12.7 k
+//   many rows                 matrix and vector work in turn at the clock that the power limit leaves (1.8 GHz): 990 us for 13.1 k
 //                             tokens of 32 heads of 128 behind 4096, 920 TFLOP/s (products alone, without the exponentials, 652 us);
 //                             head dim 64: the exponentials, 40 us for 4 k tokens of 16 heads behind 1000
 template <class T, int HD, bool VT, bool TWO>
