@@ -452,13 +452,13 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
     const int early = min(np, NS);
     for (int i = 0; i < early; ++i) issue(i);
     if (in_lds) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    // one search for all: lanes 0 .. 31 for their rows, lane 32 for the tile's first token, the others for the last one that belongs to a text
+    // one search for all: lanes 0 .. 31 for their rows, lane 32 for the tile's first token that belongs to a text, the others for the last
     int lo, hi;
     bool live;
     const int t_last = quotient(min(r0 + 32 * NW, rows) - 1, a.G, a.r_G), t_first = quotient(r0, a.G, a.r_G);
     auto search = [&](auto cu_q, auto cu_k) {
-        const int end = a.cu_q ? min(cu_q[a.n_texts] - 1, t_last) : t_last;
-        live = prompt_own_range(a, cu_q, cu_k, half ? (li ? end : t_first) : token, lo, hi);
+        const int end = a.cu_q ? min(cu_q[a.n_texts] - 1, t_last) : t_last, begin = a.cu_q ? max(cu_q[0], t_first) : t_first;
+        live = prompt_own_range(a, cu_q, cu_k, half ? (li ? end : begin) : token, lo, hi);
     };
     typedef const __attribute__((address_space(3))) int *lds_ints;
     if (in_lds) search((lds_ints)s_cu[0], (lds_ints)s_cu[1]);

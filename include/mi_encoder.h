@@ -204,7 +204,7 @@ typedef struct mi_prompt_attn {
     const int32_t *cu_q, *cu_k;      /* device, [n_texts + 1], not decreasing; both NULL: one text */
     int32_t causal;
     float scale;                     /* 1 / sqrt(head_dim) as a rule */
-    int32_t zero_rest;               /* tokens behind the last text: 0 left as they are, 1 zeros */
+    int32_t zero_rest;               /* tokens of no text, in front of the first and behind the last: 0 left as they are, 1 zeros */
     int32_t reserved;                /* 0 */
     void *workspace;                 /* device, 16-byte aligned, mi_prompt_attention_workspace bytes; not shared by calls that can overlap */
     int64_t workspace_bytes;

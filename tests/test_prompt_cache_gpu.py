@@ -498,6 +498,23 @@ def test_split_keys_and_rows_without_any(pc, prompt, first):
     close(out[:-tail][keep], o[keep], b[keep])
 
 
+@pytest.mark.parametrize("prompt,front,n", [(0, 5, 3), (70, 5, 3), (70, 200, 3), (0, 33, 400)])
+def test_rows_in_front_of_the_first_text(pc, prompt, front, n):
+    """bounds that begin behind 0: the rows and keys in front belong to no text"""
+    lens = [2, n, 40]
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, HF, 6, 3, 64, prompt, lens, [0, 9, 1])
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    wide = lambda t, m: torch.cat([torch.full_like(t[:1], math.nan).expand(m, -1, -1), t])
+    qq, kk, vv = wide(q, front), wide(k, 11), wide(v, 11)
+    out = torch.full_like(qq, 7.0)
+    bounds = dev([c + front for c in cu_q]), dev([c + 11 for c in cu_k])
+    cache.attention(e, 1, qq, kk, vv, *bounds, out=out)
+    assert (out[:front] == 7.0).all()
+    close(out[front:], o, b)
+    fresh = cache.attention(e, 1, qq, kk, vv, *bounds)
+    assert (fresh[:front] == 0).all() and torch.equal(fresh[front:], out[front:])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_both_forms_of_the_probabilities(pc, dtype):
     """few rows keep the probabilities in two parts: the error is the output's rounding alone; many rows keep one part"""
