@@ -232,6 +232,30 @@ def test_what_is_masked_may_hold_anything(pc, dtype, heads, kv, hd, prompt, lens
     assert torch.isnan(out[~ok]).all()
 
 
+@pytest.mark.parametrize("prompt,lens", [(300, [40, 3, 60]), (2000, [1, 1, 1])])
+def test_prompts_that_hold_no_numbers(pc, prompt, lens):
+    """infinities and NaN that rows do see: those rows are not finite, the others right"""
+    for what, where in ((math.nan, "v"), (math.inf, "v"), (math.nan, "k")):
+        cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 8, 2, 128, prompt, lens)
+        o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+        bad = (pv if where == "v" else pk)[None, prompt - 7:prompt - 6].clone()
+        bad[..., 1, 5] = what                                 # key head 1, dim 5
+        other = (pk if where == "v" else pv)[None, prompt - 7:prompt - 6]
+        cache.write(e, bad if where == "k" else other, bad if where == "v" else other, prompt - 7, layer=1)
+        v[cu_k[1] - 1] = math.nan                             # and a text's last value: only its last token sees it
+        out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+        last = cu_q[1] - 1
+        keep = [t for t in range(cu_q[-1]) if t != last]
+        close(out[keep][:, :4], o[keep][:, :4], b[keep][:, :4])
+        assert out[last].isnan().all()
+        if where == "k":
+            assert out[:, 4:].isnan().all()
+        else:                                                 # (an infinity stays one behind a masked NaN)
+            assert (out[keep][:, 4:, 5].isnan() if what != what else out[keep][:, 4:, 5] == what).all()
+            dims = [d for d in range(128) if d != 5]
+            close(out[keep][:, 4:][..., dims], o[keep][:, 4:][..., dims], b[keep][:, 4:][..., dims])
+
+
 def test_extreme_scores(pc):
     """scores far apart (a one-hot softmax), all equal, and a maximum that grows all along the prompt"""
     for dtype in (BF, HF):
