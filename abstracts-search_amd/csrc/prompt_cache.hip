@@ -255,7 +255,7 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
 
 // How a call is cut up: tiles of 128 rows of a key head, and where these do not fill the chip the keys `splits` ways, so that there
 // is a workgroup for each of the 256 CUs -- two, if each still has eight chunks of 64 keys or more: 50 us with 64 splits of the 1024
-// chunks of four tokens behind 65 500, 66 with 32; but 32 with 32 splits of the 82 chunks of 64 single tokens behind 2048, 27 with 16,
+// chunks of four tokens behind 65 500, 66 with 32; but 32 with 32 splits of the 82 chunks of 64 single tokens behind 2048, 26 with 16,
 // because every split's partials are written and read again.  At least two chunks each, as far as there are two: the join costs as
 // much as they do (3 us).
 struct Plan {
@@ -289,7 +289,7 @@ void attention_launch(const PromptArgs &a, const Plan &p, hipStream_t st) {
     MI_HIP(hipGetLastError());
     if (p.splits > 1) {
         constexpr int per_wg = 256 / (HD / 4);                                    // groups of lanes
-        if (p.splits > 8) hipLaunchKernelGGL((prompt_join_kernel<T, HD, 8>), dim3((unsigned)((p.rows + per_wg / 8 - 1) / (per_wg / 8))), dim3(256), 0, st, a);
+        if (p.splits > 8) hipLaunchKernelGGL((prompt_join_kernel<T, HD, 4>), dim3((unsigned)((p.rows + per_wg / 4 - 1) / (per_wg / 4))), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((prompt_join_kernel<T, HD, 1>), dim3((unsigned)((p.rows + per_wg - 1) / per_wg)), dim3(256), 0, st, a);
         MI_HIP(hipGetLastError());
     }

@@ -328,8 +328,8 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 // longer on 4 k tokens of 16 heads behind 1000.
 // What bounds it, and what it takes with its join, launches included:
 //   few rows, short prompt    latency: launch, arguments, bounds and Q, first page, two chunks, store; 8.9 us (10 tokens behind 37)
-//   few rows, long prompt     reading the pages: 57 us for the 269 MB of 65 500 tokens (the kernel 47: 5.7 TB/s), 25.6 us for 64
-//                             single tokens with pasts (35 MB) behind 2048: 18 + 7.5 for the partials of 16 splits
+//   few rows, long prompt     reading the pages: 57 us for the 269 MB of 65 500 tokens (the kernel 47: 5.7 TB/s); 24 us for 64
+//                             single tokens with pasts (35 MB) behind 2048: 18 + 5.7 for the partials of 16 splits
 //   many rows                 matrix and vector work in turn at the clock that the power limit leaves (1.8 GHz): 990 us for 13.1 k
 //                             tokens of 32 heads of 128 behind 4096, 920 TFLOP/s (products alone, without the exponentials, 652 us);
 //                             head dim 64: the exponentials, 40 us for 4 k tokens of 16 heads behind 1000
@@ -633,9 +633,10 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
 }
 
 // the splits' partials of a row -> the output: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  HD / 4 lanes hold four dims each; PAR
-// such groups take every PAR-th split of a row (8 where there are more than 8 splits: one group would go through them as one chain
-// of loads, 34 us at 64 splits) and meet in LDS, always in the same order.  Bound by latency (4.2 us for 128 rows x 64 splits of
-// 128 dims) and by the L2s' 17 MB of partials (7.3 us for 2048 rows x 16 splits: 2.3 TB/s).
+// such groups take every PAR-th split of a row and meet in LDS, always in the same order.  One group up to 8 splits: all of its loads
+// are in flight at once (128 single tokens: 31 us with their tiles, 33 with four groups); four beyond, where one would go through them
+// as a chain (34 us at 64 splits) and eight are too many workgroups (64 single tokens behind 2048: 26.8 instead of 25.5).  Bound by
+// latency (5.2 us for 128 rows x 64 splits of 128 dims) and by the L2s' 17 MB of partials (5.7 us for 2048 rows x 16 splits: 3 TB/s).
 template <class T, int HD, int PAR>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR / PAR;                           // lanes of a group, rows of a workgroup
