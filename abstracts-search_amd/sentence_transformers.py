@@ -409,8 +409,8 @@ class SentenceTransformer:
         `prompt`: the string that `encode(prompt=...)` puts in front of every text, or a list of token ids; `prompt_name`: one of
         `prompts` (None: the default prompt).  Causal models only -- in a bidirectional one (stella, gte-Qwen2) the prompt's
         hidden states depend on the text behind it.  Returns how many tokens are held; the embeddings are the same to bf16
-        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before, and so is a single query of at
-        most 32 tokens with its prompt (that is faster).  A prompt that begins as one that is cached shares its pages.
+        rounding.  A text whose tokens do not begin with a cached prompt is encoded as before, and so are few texts behind a
+        short prompt (`prompt_break_even`: that is faster).  A prompt that begins as one that is cached shares its pages.
         `load_weights` drops all of them."""
         import torch
         if not self.config.get("causal"):
@@ -454,6 +454,13 @@ class SentenceTransformer:
     # Embeddings do not depend on which sequences share a pass beyond bf16 / f32 rounding order (tests: batching
     # invariance).  `token_budget = None`: passes of exactly `batch_size` length-sorted sequences.
     token_budget = 32768
+    # Texts behind a cached prompt that make one pass of the same cost with the prompt's tokens as without go without the cache: up to
+    # 48 tokens in all (the query-time path streams every weight once either way, and may have the attention inside its O
+    # projection: a query of 31 tokens 1.09 ms, of its own 11 behind 20 cached ones 1.21), or more than 64 of their own and up to 384
+    # in all (passes of 70 to 400 tokens cost 2.7 - 3.3 ms, by how their rows fall on the tiles: 8 texts of 15 tokens behind 24 2.71
+    # against 3.19 cached, one of 100 behind 200 3.18 against 3.39; but of 60 behind 200 3.10 against 2.40, four of 40 behind 60 3.14
+    # against 2.83, 16 of 15 behind 32 3.50 against 3.20).
+    prompt_break_even = (48, 64, 384)
 
     def _passes(self, order, token_lists, batch_size):
         """the sorted sequence indices cut into forward passes: at most `batch_size` sequences (None: no bound) and
@@ -491,12 +498,14 @@ class SentenceTransformer:
             behind = [self._behind(t) for t in token_lists]
             for i, (_, handle) in enumerate(behind):
                 by.setdefault(handle, []).append(i)
+            few, from_, to = self.prompt_break_even
             for handle, members in list(by.items()):
-                # one query of at most 32 tokens with its prompt: the query-time path, with the attention inside its O projection, is
-                # faster over all of them (1.09 ms) than over the query's own behind the cached prompt (1.21 ms)
-                if handle is not None and len(members) == 1 and len(token_lists[members[0]]) <= 32:
-                    behind[members[0]] = (0, None)
+                total = sum(len(token_lists[i]) for i in members)
+                own = total - len(members) * behind[members[0]][0]
+                if handle is not None and (total <= few or from_ < own and total <= to):
                     by.setdefault(None, []).extend(by.pop(handle))
+                    for i in members:
+                        behind[i] = (0, None)
             token_lists = [t[k:] for t, (k, _) in zip(token_lists, behind)]
             groups = list(by.items())
         for handle, members in groups:

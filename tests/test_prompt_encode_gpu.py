@@ -16,6 +16,11 @@ def st():
     return m
 
 
+@pytest.fixture(autouse=True)
+def cached_whatever_it_costs(st, monkeypatch):
+    monkeypatch.setattr(st.SentenceTransformer, "prompt_break_even", (0, 0, 0))
+
+
 @pytest.fixture(scope="module")
 def tiny():
     from oracle import encoder_oracle as E
@@ -48,8 +53,7 @@ def test_prompted_against_the_oracle(st, tiny, prompt_len, lens):
     p0 = st.debug_counter("prompted_passes")
     assert model.cache_prompt(prompt) == prompt_len
     e = model.encode_tokens(toks, normalize_embeddings=True)
-    alone = len(toks) == 1 and len(toks[0]) <= 32                 # (one short query: all of it through the query-time path)
-    assert st.debug_counter("prompted_passes") == p0 + 1 + (not alone)   # the prompt's own pass and one for the texts
+    assert st.debug_counter("prompted_passes") == p0 + 2         # the prompt's own pass and one for the texts
     ref = oracle_encode(cfg, W, toks)
     same(e, ref, 1e-3)
     same(e, plain, 1e-3)
@@ -60,6 +64,36 @@ def test_prompted_against_the_oracle(st, tiny, prompt_len, lens):
     p1 = st.debug_counter("prompted_passes")
     assert np.array_equal(plain, model.encode_tokens(toks, normalize_embeddings=True))
     assert st.debug_counter("prompted_passes") == p1
+
+
+def test_few_texts_behind_a_short_prompt_go_without_it(st, tiny, monkeypatch):
+    """where a pass over all tokens costs no more than one over the texts' own, the cache is not used (and the result is the plain one's)"""
+    cfg, W = tiny
+    monkeypatch.undo()
+    assert st.SentenceTransformer.prompt_break_even == (48, 64, 384)
+    rng = np.random.default_rng(4)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    ids = lambda n: rng.integers(0, cfg.vocab_size, n).tolist()
+    short, long = ids(20), ids(100)
+    #                  texts             used
+    for prompt, lens, cached in ((short, [11], False), (short, [28], False), (short, [29], True), (short, [15] * 8, False), (short, [60], True),
+                                 (short, [14] * 16, True), (long, [5], True), (long, [65], False), (long, [64], True), (long, [60] * 6, True)):
+        toks = [prompt + ids(n) for n in lens]
+        plain = model.encode_tokens(toks, normalize_embeddings=True)
+        model.cache_prompt(prompt)
+        p0 = st.debug_counter("prompted_passes")
+        got = model.encode_tokens(toks, normalize_embeddings=True)
+        assert st.debug_counter("prompted_passes") == p0 + cached, (len(prompt), lens)
+        same(got, plain, 1e-3)
+        assert cached or np.array_equal(got, plain)
+        model.drop_prompts()
+    # groups of either kind in one call, results in their places
+    model.cache_prompt(short)
+    model.cache_prompt(long)
+    toks = [short + ids(10), ids(30), long + ids(7), ids(3), long + ids(2)]
+    p0 = st.debug_counter("prompted_passes")
+    same(model.encode_tokens(toks, normalize_embeddings=True), oracle_encode(cfg, W, toks), 1e-3)
+    assert st.debug_counter("prompted_passes") == p0 + 1
 
 
 @pytest.mark.parametrize("knob", [None, "MI_NO_FEW", "MI_NO_FEW_QKV8", "MI_NO_ROPE_FUSE"])
