@@ -113,9 +113,11 @@ struct mi_prompt_cache {
     void reads(Entry &e, void *stream, bool cap) {
         if (cap || stream != e.home) e.foreign = true;
     }
-    // src[j] -> dst[j]; into: the new entry that the pages dst make up; kids, parent: the new entries that fork `parent`
+    // src[j] -> dst[j]; into: the new entry that the pages dst make up; kids, parent: the new entries that fork `parent`; move: the pages
+    // leave src, whose numbers in all tables become dst's (ascending, and no page goes up: a word that one launch of the list has
+    // rewritten is below all that later ones look for)
     void copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st, int32_t into = -1,
-                    const int32_t *kids = nullptr, int32_t parent = -1, int shared = 0);
+                    const int32_t *kids = nullptr, int32_t parent = -1, int shared = 0, bool move = false);
     void check_room(const Entry &e, int32_t n) const {
         const int64_t most = cfg.max_tokens ? cfg.max_tokens : (int64_t)table_ld * PC_PAGE;
         if (n < 0 || (int64_t)e.len + n > most) throw Error("prompt cache: an entry holds at most " + std::to_string(most) + " tokens");
@@ -136,19 +138,20 @@ struct mi_prompt_cache {
         e.len += n;
     }
     void set_table(int32_t e, int at_, const int32_t *val, int n, hipStream_t st);
-    void remap(const int32_t *src, const int32_t *dst, int n, hipStream_t st);
 };
 
 void mi_prompt_cache::copy_pages(const bf16_t *from, bf16_t *to, const int32_t *src, const int32_t *dst, int n, int rows, hipStream_t st, int32_t into,
-                                 const int32_t *kids, int32_t parent, int shared) {
+                                 const int32_t *kids, int32_t parent, int shared, bool move) {
     PcCopyArgs a{};
     a.from = from; a.to = to; a.page_stride = page_stride; a.segs = cfg.n_layers * cfg.n_kv_heads * 2; a.hd = cfg.head_dim; a.rows = rows;
     a.tables = tables.get<int32_t>(); a.ld = table_ld; a.shared = shared;
     if (kids) a.parent_table = table(parent);
+    if (move) a.remap_words = (int64_t)cfg.max_entries * table_ld;
     constexpr int most = sizeof a.src / sizeof a.src[0];
     const int64_t words = (int64_t)a.segs * rows * cfg.head_dim / 8;
     for (int j0 = 0; j0 < n; j0 += most) {
         const int m = std::min(most, n - j0);
+        a.n = m;
         std::copy(src + j0, src + j0 + m, a.src);
         std::copy(dst + j0, dst + j0 + m, a.dst);
         if (kids) std::copy(kids + j0, kids + j0 + m, a.kid);
@@ -165,19 +168,6 @@ void mi_prompt_cache::set_table(int32_t e, int at_, const int32_t *val, int n, h
         a.dst = table(e) + at_ + i0;
         std::copy(val + i0, val + i0 + a.n, a.val);
         hipLaunchKernelGGL(pc_table_kernel, dim3(1), dim3(256), 0, st, a);
-        MI_HIP(hipGetLastError());
-    }
-}
-
-void mi_prompt_cache::remap(const int32_t *src, const int32_t *dst, int n, hipStream_t st) {
-    PcRemapArgs a{};
-    a.tables = tables.get<int32_t>();
-    a.words = (int64_t)cfg.max_entries * table_ld;
-    for (int j0 = 0; j0 < n; j0 += 480) {
-        a.n = std::min(480, n - j0);
-        std::copy(src + j0, src + j0 + a.n, a.src);
-        std::copy(dst + j0, dst + j0 + a.n, a.dst);
-        hipLaunchKernelGGL(pc_remap_kernel, dim3((unsigned)std::min<int64_t>(1024, (a.words + 255) / 256)), dim3(256), 0, st, a);
         MI_HIP(hipGetLastError());
     }
 }
@@ -563,8 +553,7 @@ int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
         for (const std::vector<int32_t> *pages : {&dst, &src})
             for (int32_t p : *pages) cross = cross || (c->tag[p] != ANY && c->tag[p] != stream);
         if (cross) c->wait_all();
-        c->copy_pages(c->pages, c->pages, src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream));
-        c->remap(src.data(), dst.data(), (int)src.size(), as_stream(stream));
+        c->copy_pages(c->pages, c->pages, src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream), -1, nullptr, -1, 0, true);
         std::vector<int32_t> to(n);
         for (int32_t p = 0; p < n; ++p) to[p] = p;
         for (size_t j = 0; j < src.size(); ++j) {
@@ -601,9 +590,7 @@ int mi_prompt_cache_resize(mi_prompt_cache *c, void *pages, int32_t n_pages, voi
             MI_HIP(hipMemset(pages, 0, bytes));
         }
         c->wait_all();
-        c->copy_pages(c->pages, static_cast<bf16_t *>(pages), src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream));
-        // (ascending, and no page goes up: a word that one launch of the list has rewritten is below all that later ones look for)
-        c->remap(src.data(), dst.data(), (int)src.size(), as_stream(stream));
+        c->copy_pages(c->pages, static_cast<bf16_t *>(pages), src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream), -1, nullptr, -1, 0, true);
         c->wait_all();
         std::vector<int32_t> to(c->cfg.n_pages, 0), ref(n_pages, 0);
         for (size_t j = 0; j < src.size(); ++j) { to[src[j]] = dst[j]; ref[dst[j]] = c->ref[src[j]]; }

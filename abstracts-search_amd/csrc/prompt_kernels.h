@@ -745,7 +745,8 @@ __global__ void __launch_bounds__(256) pc_write_kernel(PcWriteArgs a) {
 }
 
 // the first `rows` rows of every (layer, key head, K / V) of page src[j] -> page dst[j].  grid (blocks, jobs): a thread takes four
-// words, so that a launch of a few pages fills the chip too.  200 pages of 28 layers (734 MB read and written): 128 us, 5.7 TB/s; 200
+// words, so that a launch of a few pages fills the chip too.  200 pages of 28 layers (734 MB read and written): 128 us, 5.7 TB/s, with
+// the words of the tables where the pages move (a launch of their own took 4.6 us for 200 moves in 1600 words, latency); 200
 // copies of 40 rows of one page: 35 us; four: 4.0.
 struct PcCopyArgs {
     const bf16_t *from;
@@ -758,6 +759,10 @@ struct PcCopyArgs {
     const int32_t *parent_table;
     int64_t ld;
     int shared;
+    // pages that move: remap_words words of all tables, in which src[j] -> dst[j] (src ascending; words behind an entry's length may
+    // change too, nothing reads them).  Neither the copies nor the words wait for the other.
+    int n;
+    int64_t remap_words;
     int32_t src[320], dst[320], kid[320];
 };
 __global__ void __launch_bounds__(256) pc_copy_kernel(PcCopyArgs a) {
@@ -766,6 +771,22 @@ __global__ void __launch_bounds__(256) pc_copy_kernel(PcCopyArgs a) {
         if (a.parent_table) {
             int32_t *t = a.tables + a.kid[blockIdx.y] * a.ld;
             for (int i = threadIdx.x; i <= a.shared; i += 256) t[i] = i < a.shared ? a.parent_table[i] : a.dst[blockIdx.y];
+        }
+    }
+    const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256;
+    if (first < a.remap_words) {                              // (a word each thread, as far as they go, and a search in LDS)
+        __shared__ int32_t src[320], dst[320];
+        for (int i = threadIdx.x; i < a.n; i += 256) { src[i] = a.src[i]; dst[i] = a.dst[i]; }
+        __syncthreads();
+        for (int64_t i = first + threadIdx.x; i < a.remap_words; i += (int64_t)gridDim.y * gridDim.x * 256) {
+            const int32_t v = a.tables[i];
+            int lo = 0, n = a.n;
+            while (n > 1) {
+                const int half = n >> 1;
+                if (src[lo + half] <= v) lo += half;
+                n -= half;
+            }
+            if (src[lo] == v) a.tables[i] = dst[lo];
         }
     }
     const int per = a.rows * a.hd / 8;                        // 16-byte words of a segment
@@ -789,30 +810,6 @@ __global__ void __launch_bounds__(256) pc_fork_kernel(PcForkArgs a) {
     const int32_t *p = a.tables + a.parent * a.ld;
     int32_t *t = a.tables + a.entry[blockIdx.x] * a.ld;
     for (int i = threadIdx.x; i < a.shared; i += 256) t[i] = p[i];
-}
-
-// page numbers src[j] -> dst[j] in every table (src ascending; words behind an entry's length may change too, nothing reads them);
-// a word each thread and a search in LDS: 4.6 us for 200 moves in 4 tables of 400 pages, latency
-struct PcRemapArgs {
-    int32_t *tables;
-    int64_t words;
-    int n;
-    int32_t src[480], dst[480];
-};
-__global__ void __launch_bounds__(256) pc_remap_kernel(PcRemapArgs a) {
-    __shared__ int32_t src[480], dst[480];
-    for (int i = threadIdx.x; i < a.n; i += 256) { src[i] = a.src[i]; dst[i] = a.dst[i]; }
-    __syncthreads();
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.words; i += (int64_t)gridDim.x * 256) {
-        const int32_t v = a.tables[i];
-        int lo = 0, n = a.n;
-        while (n > 1) {
-            const int half = n >> 1;
-            if (src[lo + half] <= v) lo += half;
-            n -= half;
-        }
-        if (src[lo] == v) a.tables[i] = dst[lo];
-    }
 }
 
 }  // namespace mipc
