@@ -246,8 +246,9 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
 // How a call is cut up: tiles of 128 rows of a key head, and where these do not fill the chip the keys `splits` ways, so that there
 // is a workgroup for each of the 256 CUs -- two, if each still has eight chunks of 64 keys or more: 50 us with 64 splits of the 1024
 // chunks of four tokens behind 65 500, 66 with 32; but 32 with 32 splits of the 82 chunks of 64 single tokens behind 2048, 26 with 16,
-// because every split's partials are written and read again.  At least two chunks each, as far as there are two: the join costs as
-// much as they do (3 us).
+// because every split's partials are written and read again.  Up to 256 rows a split may be one chunk, beyond it is two at least (ten
+// tokens of 12 heads behind 400: 12.1 us with 8 splits of one, 13.2 with 4 of two; but 30 single tokens of 28 heads behind 400 16.6 with
+// 12 splits, 13.6 with 7); up to four chunks go unsplit, where the join costs as much as they do (behind 150: 11.7 us, in two 13.0).
 struct Plan {
     int splits, tiles;
     int64_t rows;                        // of all key heads
@@ -263,7 +264,7 @@ Plan plan_of(const PromptArgs &a, int hd) {
     // chunks that a tile goes through: the prompt's, and its texts' share of the own keys
     const int64_t wgs = (int64_t)p.tiles * a.n_kv, own = a.n_keys * std::min<int64_t>(per_head, R) / per_head;
     const int64_t chunks = (a.P + PC_PAGE - 1) / PC_PAGE + (own + PC_PAGE - 1) / PC_PAGE, target = chunks * wgs >= 8 * 512 ? 512 : 256;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(target / wgs, chunks / 2));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(target / wgs, chunks < 5 ? 1 : p.rows <= 256 ? chunks : chunks / 2));
     p.o_bytes = p.splits > 1 ? p.splits * p.rows * hd * 4 : 0;
     p.bytes = p.splits > 1 ? p.o_bytes + p.splits * p.rows * 8 : 0;
     return p;
