@@ -263,8 +263,8 @@ class PromptCache:
         cu_k[i + 1] (cu_k None: the same as cu_q; both None: one text).  With more keys than queries the first keys are the
         text's past: one query per text is the form for single tokens.  Every query sees the whole prompt; `causal`: of its
         own text the keys up to itself, otherwise all.  A query that sees nothing gets zeros.  scale: 1 / sqrt(head_dim) if
-        None.  out: written in place if given (tokens of no text, in front of the first or behind the last, keep what they hold; in a new output they are
-        zeros).  Inference only: no gradient."""
+        None.  out: written in place if given (tokens of no text, in front of the first or behind the last, keep what they
+        hold; in a new output they are zeros).  Inference only: no gradient."""
         import torch
         hd, kv, dtype, device = self.head_dim, self.n_kv_heads, self.dtype, self.device
         if q.dim() != 3 or q.shape[2] != hd:
