@@ -167,4 +167,32 @@ struct DeviceGuard {
     }
 };
 
+// While another thread captures a graph, a call of this one that allocates, frees or waits fails by default and ends that capture.
+// Inside this scope it does neither (hipDeviceSynchronize and the synchronous copies and fills of the null stream excepted).
+struct BesideCaptures {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    BesideCaptures() { swap(); }
+    ~BesideCaptures() { swap(); }
+    BesideCaptures(const BesideCaptures &) = delete;
+    BesideCaptures &operator=(const BesideCaptures &) = delete;
+
+private:
+    void swap() {
+        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) (void)hipGetLastError();
+    }
+};
+
+// Waits for all work on the current device, beside other threads' captures too: hipFree waits for the device (its documentation: an
+// implicit hipDeviceSynchronize).  2.6 us on an idle device, where hipDeviceSynchronize takes 0.4.
+inline void wait_for_device() {
+    BesideCaptures beside;
+    void *p = nullptr;
+    if (hipMalloc(&p, 256) != hipSuccess) {                  // no memory left: the plain wait
+        (void)hipGetLastError();
+        MI_HIP(hipDeviceSynchronize());
+        return;
+    }
+    MI_HIP(hipFree(p));
+}
+
 }  // namespace mi

@@ -722,6 +722,7 @@ struct mi_encoder {
         DevBuf sum;                          // f32 [hidden]: the tokens' final-norm hidden states (bf16 values, as the pooling sees them)
         ~Prompt() {
             if (entry < 0) return;
+            BesideCaptures beside;               // (an error here would leave the entry in the pool for good)
             int prev = 0;
             (void)hipGetDevice(&prev);
             (void)hipSetDevice(device);
@@ -1732,6 +1733,7 @@ int mi_encoder_cache_prompt(mi_encoder *h, int n, const int32_t *ids, int32_t *p
         MI_REQUIRE(c.causal, "cached prompts need a causal model: in a bidirectional one a prompt's hidden states depend on the text behind it");
         MI_REQUIRE(n >= 1 && n < c.max_seq_len, "a cached prompt holds 1 .. max_seq_len - 1 tokens");
         DeviceGuard dg(h->device);
+        BesideCaptures beside;
         hipStream_t st = as_stream(stream);
         std::lock_guard<std::mutex> pl(h->prompts_mu);
         constexpr int max_prompts = 256;

@@ -77,7 +77,7 @@ struct mi_prompt_cache {
     int32_t *table(int32_t e) const { return tables.get<int32_t>() + (int64_t)e * table_ld; }
 
     void wait_all() {                    // everything issued so far is done: whatever is free is free for every stream
-        MI_HIP(hipDeviceSynchronize());
+        wait_for_device();
         std::fill(tag.begin(), tag.end(), ANY);
         for (Entry &e : entries)
             if (!e.live) e.slot_tag = ANY;
@@ -173,6 +173,12 @@ void mi_prompt_cache::set_table(int32_t e, int at_, const int32_t *val, int n, h
 }
 
 namespace {
+
+// zeros by a kernel, which a capture in another thread does not mind
+void zero(void *p, size_t bytes, hipStream_t st) {
+    hipLaunchKernelGGL(pc_zero_kernel, dim3((unsigned)std::min<size_t>(4096, bytes / 4096 + 1)), dim3(256), 0, st, static_cast<uint32_t *>(p), (int64_t)(bytes / 4));
+    MI_HIP(hipGetLastError());
+}
 
 // memory that a kernel on `device` may use
 bool on_device(const void *p, int device) {
@@ -355,13 +361,14 @@ int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pag
         c->page_stride = c->layer_stride * g.n_layers;
         c->table_ld = g.max_tokens ? (int)(((int64_t)g.max_tokens + PC_PAGE - 1) / PC_PAGE) : g.n_pages;
         const size_t bytes = (size_t)c->page_stride * 2 * g.n_pages, tbytes = (size_t)g.max_entries * c->table_ld * 4;
+        BesideCaptures beside;
         if (!pages) {                    // zeros: what a reserved token holds before it is written is at least finite
             pages = c->own.reserve(bytes);
-            MI_HIP(hipMemset(pages, 0, bytes));
+            zero(pages, bytes, nullptr);
         }
         c->pages = static_cast<bf16_t *>(pages);
-        MI_HIP(hipMemset(c->tables.reserve(tbytes), 0, tbytes));   // (every word of a table is a page number, whatever is read)
-        MI_HIP(hipDeviceSynchronize());
+        zero(c->tables.reserve(tbytes), tbytes, nullptr);          // (every word of a table is a page number, whatever is read)
+        wait_for_device();
         c->ref.assign(g.n_pages, 0);
         c->tag.assign(g.n_pages, ANY);
         c->free_pages.reset(g.n_pages, 0);
@@ -374,7 +381,8 @@ int mi_prompt_cache_destroy(mi_prompt_cache *c) {
     return guard([&] {
         if (!c) return;
         DeviceGuard dg(c->device);
-        MI_HIP(hipDeviceSynchronize());
+        BesideCaptures beside;
+        wait_for_device();
         delete c;
     });
 }
@@ -585,10 +593,11 @@ int mi_prompt_cache_resize(mi_prompt_cache *c, void *pages, int32_t n_pages, voi
         MI_REQUIRE(n_pages <= 0x7fffffff / PC_PAGE, "prompt cache: more than 2^31 tokens");
         MI_REQUIRE(!pages || (aligned16(pages) && on_device(pages, c->device)), "prompt cache: pages must be 16-byte aligned memory of the device");
         const size_t bytes = (size_t)c->page_stride * 2 * n_pages;
+        BesideCaptures beside;
         DevBuf own;
         if (!pages) {
             pages = own.reserve(bytes);
-            MI_HIP(hipMemset(pages, 0, bytes));
+            zero(pages, bytes, as_stream(stream));
         }
         c->wait_all();
         c->copy_pages(c->pages, static_cast<bf16_t *>(pages), src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream), -1, nullptr, -1, 0, true);

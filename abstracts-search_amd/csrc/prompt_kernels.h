@@ -799,6 +799,11 @@ __global__ void __launch_bounds__(256) pc_copy_kernel(PcCopyArgs a) {
     }
 }
 
+// words of new pages and tables: zeros
+__global__ void __launch_bounds__(256) pc_zero_kernel(uint32_t *p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
 // the tables of new entries that begin as `parent` does, its pages all full
 struct PcForkArgs {
     int32_t *tables;

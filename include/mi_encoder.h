@@ -139,6 +139,7 @@ int mi_enc_gemm_bf16(int device, int M, int N, int K, const void *A, const void 
  * reads, are given out again only after the device has been waited for.  mi_prompt_attention and mi_prompt_cache_write may be
  * captured into a graph (a replay uses the entry's length as it was at the capture; the entry must live, page moves by
  * mi_prompt_cache_compact are followed, a resize ends its use); the other calls are refused on a stream that is being captured.
+ * A capture that another thread has open is left alone: no call here fails because of it or ends it, also where it waits.
  * ------------------------------------------------------------------------------------------------------------------- */
 #define MI_PROMPT_PAGE 64
 

@@ -702,3 +702,72 @@ def test_refusals(pc):
     small.reserve(x, 100)
     o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)    # nothing of this has changed the prompt
     close(cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k)), o, b)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# calls at the edges
+# ---------------------------------------------------------------------------------------------------------------
+class OpenCapture:
+    """another thread captures a stream in global mode while the body runs; `ended`: what hipStreamEndCapture returned"""
+
+    def __enter__(self):
+        import ctypes
+        import threading
+        hip, V = ctypes.CDLL("libamdhip64.so"), ctypes.c_void_p
+        self.leave, opened, side = threading.Event(), threading.Event(), torch.cuda.Stream()
+
+        def run():
+            self.began = hip.hipStreamBeginCapture(V(side.cuda_stream), 0)
+            opened.set()
+            self.leave.wait(60)
+            self.ended = hip.hipStreamEndCapture(V(side.cuda_stream), ctypes.byref(V()))
+            hip.hipGetLastError()
+
+        self.thread = threading.Thread(target=run, daemon=True)
+        self.thread.start()
+        assert opened.wait(60) and self.began == 0
+        return self
+
+    def __exit__(self, *exc):
+        self.leave.set()
+        self.thread.join()
+
+
+def test_captures_of_other_threads_are_left_alone(pc):
+    """whatever waits for the device, allocates or clears works beside a capture in another thread, waits in earnest, and lets it be
+    (torch's own allocator does not: what it hands out inside was held before)"""
+    cache = pc.PromptCache(1, 1, 64, 4, max_entries=4)
+    kv, q = torch.randn(1, 64, 1, 64, device="cuda", dtype=BF), torch.randn(1, 2, 64, device="cuda", dtype=BF)
+    side, nothing, got = torch.cuda.Stream(), kv * 0, [torch.empty_like(q) for _ in range(3)]
+
+    def read_elsewhere(e, out):                               # from here on whoever takes e's pages has to wait for `side`
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            cache.attention(e, 0, q, out=out)
+
+    low, e = cache.new(), cache.new()
+    for x in (low, e):
+        cache.extend(x, kv, kv)
+    want = cache.attention(e, 0, q)
+    read_elsewhere(e, got[0])
+    torch.zeros((6, 1, 1, 2, 64, 64), dtype=BF, device="cuda")
+    torch.cuda.synchronize()
+    with OpenCapture() as c:
+        read_elsewhere(e, got[0])
+        cache.free(low)
+        assert cache.compact() == 1 and cache.table(e) == [0]                     # waits for `side`
+        read_elsewhere(e, got[1])
+        cache.resize(6)
+        read_elsewhere(e, got[2])
+        cache.free(e)
+        e = cache.new()
+        cache.extend(e, nothing, nothing)
+        raw = pc.c_void_p()                                                        # (pages that the library allocates and clears)
+        pc._check(pc._Lib.get().mi_prompt_cache_create(pc.ctypes.byref(pc._Cfg(1, 1, 64, 1, 4, 2, 0)), 0, None, pc.ctypes.byref(raw)))
+        pc._check(pc._Lib.get().mi_prompt_cache_resize(raw, None, 9, None))
+        pc._check(pc._Lib.get().mi_prompt_cache_destroy(raw))
+    assert c.ended == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+    assert (cache.pages[cache.table(e)[0]] == 0).all()

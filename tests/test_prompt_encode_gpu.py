@@ -239,3 +239,23 @@ def test_refusals(st, tiny):
     model.load_weights({"norm.weight": W["norm.weight"]})         # (drops the prompts)
     assert run(h, ids[:3]) != 0 and not model._cached_prompts
     torch.cuda.synchronize()
+
+
+def test_prompts_come_and_go_beside_a_capture(st, tiny):
+    """another thread's open capture neither stops a prompt from being cached or dropped nor ends; what is dropped leaves the pool (of
+    512 entries: a third round would find it full)"""
+    from test_prompt_cache_gpu import OpenCapture
+    cfg, W = tiny
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    model.cache_prompt([1, 2, 3])
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for i in range(255):
+            model.cache_prompt([5, i % 50, i // 50])
+        with torch.cuda.stream(side):                         # read on another stream: its pages are waited for
+            model.encode_tokens([[5, 0, 0, 7, 9], [5, 1, 0, 3]])
+        with OpenCapture() as c:
+            model.drop_prompts()
+            model.cache_prompt([1, 2, 3])
+        assert c.ended == 0
+    assert np.isfinite(model.encode_tokens([[1, 2, 3, 4]])).all()
