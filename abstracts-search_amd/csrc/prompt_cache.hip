@@ -204,8 +204,13 @@ void write_args(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_laye
     Entry &e = c->at(entry);
     MI_REQUIRE(layer >= 0 && n_layers >= 1 && n_layers <= c->cfg.n_layers - layer, "prompt cache: layer out of range");
     MI_REQUIRE(start >= 0 && n >= 0 && n <= e.len - start, "prompt cache: tokens out of the entry's range");
-    for (int p = start / PC_PAGE; p < (start + n + PC_PAGE - 1) / PC_PAGE; ++p)
+    bool wait = false;                   // an entry that shared a page gave it up on another stream, where its reading may be under way
+    for (int p = start / PC_PAGE; p < (start + n + PC_PAGE - 1) / PC_PAGE; ++p) {
         MI_REQUIRE(c->ref[e.pages[p]] == 1, "prompt cache: tokens in a page that other entries share cannot be written");
+        void *const t = c->tag[e.pages[p]];
+        wait = wait || (t != ANY && (t != stream || capturing(stream)));         // (a replay may run on any stream)
+    }
+    if (wait) c->wait_all();
     c->reads(e, stream, capturing(stream));
     a.pages = c->pages; a.page_stride = c->page_stride; a.layer_stride = c->layer_stride; a.table = c->table(entry);
     a.layer = layer; a.n_layers = n_layers; a.start = start; a.n = n; a.n_kv = c->cfg.n_kv_heads; a.hd = c->cfg.head_dim;

@@ -164,7 +164,8 @@ int mi_prompt_cache_new(mi_prompt_cache *c, void *stream, int32_t *entry);
 int mi_prompt_cache_reserve(mi_prompt_cache *c, int32_t entry, int32_t n, void *stream);
 /* keys and values of tokens start .. start + n - 1 of an entry, layers layer .. layer + n_layers - 1.  k and v: device, the
  * cache's dtype, element (l, t, h, d) at l * layer_stride + t * token_stride + h * head_stride + d (strides in elements,
- * multiples of 8; pointers 16-byte aligned).  Pages that other entries share are refused. */
+ * multiples of 8; pointers 16-byte aligned).  Pages that other entries share are refused; reading by entries that shared one and are
+ * freed is waited for.  (Reading of this entry on other streams is the caller's to order, as with any device buffer.) */
 int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_layers, int32_t start, int32_t n,
                           const void *k, const int64_t k_strides[3], const void *v, const int64_t v_strides[3], void *stream);
 /* n more tokens and their keys and values, all layers, in one launch: reserve and write. */

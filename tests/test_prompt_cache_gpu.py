@@ -771,3 +771,35 @@ def test_captures_of_other_threads_are_left_alone(pc):
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
     assert (cache.pages[cache.table(e)[0]] == 0).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_page_that_was_shared_is_written_behind_its_readers(pc, captured):
+    """a fork reads on a stream of its own and is freed there; its parent then writes the page that both held, eagerly or in a graph:
+    behind the fork's reading"""
+    cache = pc.PromptCache(1, 1, 64, 4, max_entries=6)
+    kv, q = torch.randn(1, 64, 1, 64, device="cuda", dtype=BF), torch.randn(1, 2, 64, device="cuda", dtype=BF)
+    nothing, out, side = kv * 0, torch.empty_like(q), torch.cuda.Stream()
+    parent = cache.new()
+    cache.extend(parent, kv, kv)
+    want = cache.attention(parent, 0, q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        kid = cache.fork(parent)[0]
+        torch.cuda._sleep(20_000_000)                         # ~10 ms of this stream before it reads
+        cache.attention(kid, 0, q, out=out)
+        cache.free(kid)
+        read = torch.cuda.Event()
+        read.record()
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            cache.write(parent, nothing, nothing, 0)
+        for _ in range(3):
+            g.replay()
+    else:
+        cache.write(parent, nothing, nothing, 0)
+        assert read.query()                                   # the host came back behind the reading
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert (cache.pages[0] == 0).all()
