@@ -52,6 +52,7 @@ struct Entry {
     std::vector<int32_t> pages;
     void *home = nullptr;      // the stream it was made on
     bool foreign = false;      // other streams or a captured graph read it: freeing it waits for the device
+    int graph_from = INT32_MAX;   // captured writes (whose replays come when they come) reach its pages from this one on: never shared
     void *slot_tag = ANY;      // not live: the stream whose work may still read its table
 };
 
@@ -108,7 +109,7 @@ struct mi_prompt_cache {
     }
     void open(int32_t e, int len, std::vector<int32_t> pg, void *stream) {
         Entry &x = entries[e];
-        x.live = true; x.len = len; x.pages = std::move(pg); x.home = stream; x.foreign = false; x.slot_tag = ANY;
+        x.live = true; x.len = len; x.pages = std::move(pg); x.home = stream; x.foreign = false; x.graph_from = INT32_MAX; x.slot_tag = ANY;
     }
     void reads(Entry &e, void *stream, bool cap) {
         if (cap || stream != e.home) e.foreign = true;
@@ -204,14 +205,16 @@ void write_args(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_laye
     Entry &e = c->at(entry);
     MI_REQUIRE(layer >= 0 && n_layers >= 1 && n_layers <= c->cfg.n_layers - layer, "prompt cache: layer out of range");
     MI_REQUIRE(start >= 0 && n >= 0 && n <= e.len - start, "prompt cache: tokens out of the entry's range");
+    const bool cap = capturing(stream);
     bool wait = false;                   // an entry that shared a page gave it up on another stream, where its reading may be under way
     for (int p = start / PC_PAGE; p < (start + n + PC_PAGE - 1) / PC_PAGE; ++p) {
         MI_REQUIRE(c->ref[e.pages[p]] == 1, "prompt cache: tokens in a page that other entries share cannot be written");
         void *const t = c->tag[e.pages[p]];
-        wait = wait || (t != ANY && (t != stream || capturing(stream)));         // (a replay may run on any stream)
+        wait = wait || (t != ANY && (t != stream || cap));         // (a replay may run on any stream)
     }
     if (wait) c->wait_all();
-    c->reads(e, stream, capturing(stream));
+    if (cap && n) e.graph_from = std::min(e.graph_from, start / PC_PAGE);
+    c->reads(e, stream, cap);
     a.pages = c->pages; a.page_stride = c->page_stride; a.layer_stride = c->layer_stride; a.table = c->table(entry);
     a.layer = layer; a.n_layers = n_layers; a.start = start; a.n = n; a.n_kv = c->cfg.n_kv_heads; a.hd = c->cfg.head_dim;
 }
@@ -470,12 +473,23 @@ int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32
         Entry &e = c->at(entry);
         if (!count) return;
         const std::vector<int32_t> kids = c->pick_entries(count, stream);
-        const int rows = e.len % PC_PAGE, shared = e.len / PC_PAGE;
-        const std::vector<int32_t> own = rows ? c->pick_pages(count, stream) : std::vector<int32_t>();
+        // full pages are shared, but for those that a graph may write later; of the others one is copied as far as it is used, or several whole
+        const int pages = (int)e.pages.size(), shared = std::min(e.len / PC_PAGE, e.graph_from), each = pages - shared;
+        const int rows = each == 1 && e.len % PC_PAGE ? e.len % PC_PAGE : 0;
+        if ((int64_t)each * count > c->cfg.n_pages) throw Error("prompt cache: " + std::to_string((int64_t)each * count) + " pages needed, " + std::to_string(c->free_pages.count) + " free");
+        const std::vector<int32_t> own = c->pick_pages(each * count, stream);
+        const std::vector<int32_t> base(e.pages.begin(), e.pages.begin() + shared);
+        std::vector<std::vector<int32_t>> tables(count, base);
+        for (int j = 0; j < count; ++j) tables[j].insert(tables[j].end(), own.begin() + (int64_t)j * each, own.begin() + (int64_t)(j + 1) * each);
         hipStream_t st = as_stream(stream);
         if (rows) {
             const std::vector<int32_t> src(count, e.pages[shared]);
             c->copy_pages(c->pages, c->pages, src.data(), own.data(), count, rows, st, -1, kids.data(), entry, shared);
+        } else if (each) {
+            for (int j = 0; j < count; ++j) {
+                c->set_table(kids[j], 0, tables[j].data(), pages, st);
+                c->copy_pages(c->pages, c->pages, e.pages.data() + shared, own.data() + (int64_t)j * each, each, PC_PAGE, st);
+            }
         } else if (shared) {
             PcForkArgs a{};
             a.tables = c->tables.get<int32_t>(); a.ld = c->table_ld; a.parent = entry; a.shared = shared;
@@ -487,15 +501,12 @@ int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32
             }
         }
         c->reads(e, stream, false);
-        const std::vector<int32_t> base(e.pages.begin(), e.pages.begin() + shared);
+        const int len = e.len;
         for (int32_t p : base) c->ref[p] += count;
+        for (int32_t p : own) c->take(p);
         for (int j = 0; j < count; ++j) {
-            std::vector<int32_t> pg;
-            pg.reserve(base.size() + 1);
-            pg = base;
-            if (page) page[j] = rows ? own[j] : -1;
-            if (rows) { c->take(own[j]); pg.push_back(own[j]); }
-            c->open(kids[j], c->entries[entry].len, std::move(pg), stream);
+            if (page) page[j] = rows ? own[j] : each ? -2 : -1;
+            c->open(kids[j], len, std::move(tables[j]), stream);
             out[j] = kids[j];
         }
     });

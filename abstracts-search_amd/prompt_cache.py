@@ -173,13 +173,14 @@ class PromptCache:
         return t
 
     def fork(self, entry: int, count: int = 1) -> list[int]:
-        """`count` new entries that begin as `entry` does: its full pages are shared, the tokens of its last page copied"""
+        """`count` new entries that begin as `entry` does: its full pages are shared, the tokens of its last page (and pages that
+        a captured `write` reaches) copied"""
         if count < 0:
             raise ValueError(f"PromptCache.fork: count must not be negative, got {count}")
         out, own, moves = (c_int32 * count)(), (c_int32 * count)(), self._moves
         _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, own, self._stream()))
         kids, own = out[:], own[:]
-        if count > 1:                                # (their tables without asking for each of them)
+        if count > 1 and own[0] > -2:                # (their tables without asking for each of them)
             full = self.table(entry)
             if own[0] >= 0:
                 full.pop()

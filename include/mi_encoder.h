@@ -171,8 +171,9 @@ int mi_prompt_cache_write(mi_prompt_cache *c, int32_t entry, int32_t layer, int3
 /* n more tokens and their keys and values, all layers, in one launch: reserve and write. */
 int mi_prompt_cache_extend(mi_prompt_cache *c, int32_t entry, int32_t n, const void *k, const int64_t k_strides[3], const void *v,
                            const int64_t v_strides[3], void *stream);
-/* count new entries that begin as `entry` does: full pages are shared, the used rows of the last page are copied.  pages (may be
- * NULL): the number of each one's own last page, -1 where all pages are full. */
+/* count new entries that begin as `entry` does: full pages are shared, the used rows of the last page are copied.  (Pages that a captured
+ * mi_prompt_cache_write reaches, and all behind them, are copied too: a replay changes this entry alone.)  pages (may be NULL): the
+ * number of each one's own last page, -1 where all pages are shared, -2 where several are its own. */
 int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32_t *entries, int32_t *pages, void *stream);
 /* one new entry with pages of its own throughout. */
 int mi_prompt_cache_copy(mi_prompt_cache *c, int32_t entry, int32_t *copy, void *stream);

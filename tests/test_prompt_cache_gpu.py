@@ -803,3 +803,42 @@ def test_a_page_that_was_shared_is_written_behind_its_readers(pc, captured):
     torch.cuda.synchronize()
     assert torch.equal(out, want)
     assert (cache.pages[0] == 0).all()
+
+
+@pytest.mark.parametrize("length,at,n", [(200, 64, 10), (200, 0, 64), (128, 70, 5), (192, 10, 150), (130, 128, 2), (64, 0, 0)])
+def test_a_captured_write_changes_its_own_entry_alone(pc, length, at, n):
+    """forks taken between a graph's capture and its replays keep what they held: the pages the graph writes are theirs, not shared"""
+    cache = pc.PromptCache(2, 1, 64, 40, max_entries=12)
+    g = torch.Generator(device="cuda").manual_seed(length)
+    new = lambda m: torch.randn(2, m, 1, 64, generator=g, device="cuda").to(BF)
+    k, v, k2, v2 = new(length), new(length), new(n), new(n)
+    e = cache.new()
+    cache.extend(e, k, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.write(e, k2, v2, at)
+    held = lambda x: [cache.pages[torch.tensor(cache.table(x), device="cuda")][:, :, 0, w].transpose(0, 1).reshape(2, -1, 64)[:, :length] for w in (0, 1)]
+    same = lambda x, kk, vv: torch.equal(held(x)[0], kk[:, :, 0]) and torch.equal(held(x)[1], vv[:, :, 0])
+    kids = cache.fork(e, 3) + cache.fork(e)
+    grandkid = cache.fork(kids[0])[0]
+    full, first = length // 64, at // 64 if n else 64
+    for x in kids:                                            # what lies in front of the graph's pages is shared
+        assert cache.table(x)[:min(full, first)] == cache.table(e)[:min(full, first)]
+        assert not set(cache.table(x)[min(full, first):]) & set(cache.table(e))
+    assert cache.table(grandkid)[:full] == cache.table(kids[0])[:full]
+    for rep in range(3):
+        graph.replay()
+        kk, vv = k.clone(), v.clone()
+        kk[:, at:at + n], vv[:, at:at + n] = k2, v2
+        assert same(e, kk, vv) and all(same(x, k, v) for x in [*kids, grandkid]), rep
+        k2.mul_(-1.5)
+        if rep == 1:
+            cache.compact()
+    copy = cache.copy(e)
+    assert set(cache.table(cache.fork(copy)[0])) & set(cache.table(copy)) == set(cache.table(copy)[:full])
+    cache.free([e, copy, *kids])
+    assert same(grandkid, k, v)
+    again = cache.new()                                       # the entry's number used again: nothing of the graph's is left
+    cache.extend(again, k, v)
+    assert cache.table(cache.fork(again)[0])[:full] == cache.table(again)[:full]
