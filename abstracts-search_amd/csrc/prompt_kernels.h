@@ -215,9 +215,10 @@ __device__ void prompt_row(const PromptArgs &a, int token, int head, int64_t p0,
 // The running maximum is raised only when a row's scores pass it by 8 (in log2): p stays below 2^8, the sums are f32, and the
 // rescaling of o leaves the steady state.
 //
-// A masked key has p = 0 exactly, and 0 x (inf or NaN in its V) would be NaN: a row whose result is no finite number is done again
-// by prompt_row, which reads only what the row sees -- unless its sum is NaN from the prompt's keys alone, of which none is masked:
-// then every dim is NaN whatever follows, and a batch of such rows would take seconds.
+// A masked key has p = 0 exactly (so have the rows behind the prompt's and the texts' end, which hold the last one again), a rounding may
+// leave one of 0 or less, and 0 x (inf or NaN in V) would be NaN: a row whose result is no finite number is done again by prompt_row,
+// which reads only what the row sees and keeps its probabilities in f32 -- unless its sum is NaN: the sum is over keys that the row
+// sees, so every dim is NaN.
 // ---------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) bf16_t lds_t;
 // 64 lanes x 16 bytes from base + the lane's offset -> 1 KiB at dst (the same in every lane)
@@ -255,10 +256,10 @@ __device__ __forceinline__ const PromptArgs &args_again() {
 }
 
 // a wave's 32 rows: O^T tiles, the maxima and this half's sums -> the output, or this split's partials.  Prompt keys [p0, p1) and own
-// keys [b0, b1) are what this workgroup went through; final: rows that are not done again.
+// keys [b0, b1) are what this workgroup went through.
 template <class T, int HD>
 __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float mrow, float lrow, int row, int token, int head, int lo, int hi,
-                                              bool live, int split, int kvh, int64_t p0, int64_t p1, int64_t b0, int64_t b1, unsigned final, float *qs) {
+                                              bool live, int split, int kvh, int64_t p0, int64_t p1, int64_t b0, int64_t b1, float *qs) {
     constexpr int NDT = HD / 32, DPL = HD / 64;
     const PromptArgs &a = args_again();
     const int lane = threadIdx.x & 63, li = lane & 31, half = lane >> 5, rows = a.n_tokens * a.G;
@@ -270,8 +271,8 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
     for (int n = 0; n < NDT; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(o[n][r], 0.f, zero);
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(zero != 0.f && sees);
-    unsigned redo = (unsigned)(bad | bad >> 32) & ~final;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(zero != 0.f && lrow == lrow && sees);
+    unsigned redo = (unsigned)(bad | bad >> 32);
     const int64_t prow = ((int64_t)split * a.n_kv + kvh) * rows;                 // this split's partials of the key head
     if (row < rows && !(redo >> li & 1) && (live || a.zero_rest || a.splits > 1)) {
         if (a.splits > 1) {
@@ -614,22 +615,16 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
 
-    unsigned final = 0;
     for (int i = 0; i < n; ++i) {
-        if (i == np && i > 0) {
-            const uint64_t nan = __builtin_amdgcn_ballot_w64(lrow != lrow);
-            final = (unsigned)(nan | nan >> 32);
-            if (a.inter) { load_q(false); pin_q(); }
-        }
+        if (i == np && i > 0 && a.inter) { load_q(false); pin_q(); }
         landed(i == 0 && n > 1);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");             // everyone's pieces; the chunk before is used up
         if (i > 0 && i + 1 < n) issue(i + 1);
         const int md = mode(i);
         if (md != SKIP) product(i, md);
     }
-    if (n == np) final = ~0u;
     prompt_finish<T, HD>(o, mrow, lrow, row, token, head, lo, hi, live, split, kvh, (int64_t)p0 * KC, (int64_t)(p0 + np) * KC,
-                         (int64_t)k0 + (int64_t)o0 * KC, (int64_t)k0 + (int64_t)(o0 + n - np) * KC, final, s_q[w]);
+                         (int64_t)k0 + (int64_t)o0 * KC, (int64_t)k0 + (int64_t)(o0 + n - np) * KC, s_q[w]);
 }
 
 // the splits' partials of a row -> the output: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  HD / 4 lanes hold four dims each; PAR

@@ -842,3 +842,41 @@ def test_a_captured_write_changes_its_own_entry_alone(pc, length, at, n):
     again = cache.new()                                       # the entry's number used again: nothing of the graph's is left
     cache.extend(again, k, v)
     assert cache.table(cache.fork(again)[0])[:full] == cache.table(again)[:full]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("prompt,lens", [(37, [10]), (100, [3, 1]), (2000, [1, 1, 1]), (300, [90, 40]), (64, [5])])
+def test_an_infinity_in_the_prompts_last_value(pc, dtype, prompt, lens):
+    """a page's rows behind the prompt's end weigh nothing, whatever the last token's value is: a row that sees an infinity gets it,
+    with and without own keys, few rows and many, split or not"""
+    for what in (math.inf, -math.inf, math.nan):
+        cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, 8, 2, 128, prompt, lens)
+        o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+        none = torch.zeros(0, 2, 128, dtype=dtype, device="cuda")
+        o2, b2 = reference_many(q, pk, pv, none, none, cu_q, [0] * len(cu_q), True)
+        bad = pv[None, prompt - 1:].clone()
+        bad[..., 1, 5] = what                                 # key head 1, dim 5
+        cache.write(e, pk[None, prompt - 1:].contiguous(), bad, prompt - 1, layer=1)
+        dims = [d for d in range(128) if d != 5]
+        for out, oo, bb in ((cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k)), o, b), (cache.attention(e, 1, q, None, None, dev(cu_q)), o2, b2)):
+            close(out[:, :4], oo[:, :4], bb[:, :4])
+            close(out[:, 4:][..., dims], oo[:, 4:][..., dims], bb[:, 4:][..., dims])
+            assert (out[:, 4:, 5].isnan() if what != what else out[:, 4:, 5] == what).all(), what
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("prompt,lens,past", [(0, [30], None), (70, [9, 64, 5], None), (0, [90, 110], None), (2000, [1, 1], [70, 3])])
+def test_an_infinity_among_the_own_values(pc, dtype, prompt, lens, past):
+    """rows that see it get it (its probability is held exactly by one rounding, by both, or by none), the rows before it keep their
+    values"""
+    for what in (math.inf, -math.inf):
+        for back in (1, 2, 4):                                # the text's last key, and ones that more of its rows see
+            cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, dtype, 8, 2, 128, prompt, lens, past)
+            o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+            at = cu_k[1] - back
+            v[at, 1, 5] = what                                # key head 1, dim 5 of the first text
+            out = cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k))
+            sees = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+            sees[max(0, cu_q[1] - back):cu_q[1], 4:, 5] = True
+            assert (out[sees] == what).all(), (what, back)
+            close(out[~sees], o[~sees], b[~sees])
