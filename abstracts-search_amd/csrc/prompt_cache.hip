@@ -479,15 +479,20 @@ int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32
         if ((int64_t)each * count > c->cfg.n_pages) throw Error("prompt cache: " + std::to_string((int64_t)each * count) + " pages needed, " + std::to_string(c->free_pages.count) + " free");
         const std::vector<int32_t> own = c->pick_pages(each * count, stream);
         const std::vector<int32_t> base(e.pages.begin(), e.pages.begin() + shared);
-        std::vector<std::vector<int32_t>> tables(count, base);
-        for (int j = 0; j < count; ++j) tables[j].insert(tables[j].end(), own.begin() + (int64_t)j * each, own.begin() + (int64_t)(j + 1) * each);
+        auto pages_of = [&](int j) {
+            std::vector<int32_t> pg;
+            pg.reserve(pages);
+            pg = base;
+            pg.insert(pg.end(), own.begin() + (int64_t)j * each, own.begin() + (int64_t)(j + 1) * each);
+            return pg;
+        };
         hipStream_t st = as_stream(stream);
         if (rows) {
             const std::vector<int32_t> src(count, e.pages[shared]);
             c->copy_pages(c->pages, c->pages, src.data(), own.data(), count, rows, st, -1, kids.data(), entry, shared);
         } else if (each) {
             for (int j = 0; j < count; ++j) {
-                c->set_table(kids[j], 0, tables[j].data(), pages, st);
+                c->set_table(kids[j], 0, pages_of(j).data(), pages, st);
                 c->copy_pages(c->pages, c->pages, e.pages.data() + shared, own.data() + (int64_t)j * each, each, PC_PAGE, st);
             }
         } else if (shared) {
@@ -506,7 +511,7 @@ int mi_prompt_cache_fork(mi_prompt_cache *c, int32_t entry, int32_t count, int32
         for (int32_t p : own) c->take(p);
         for (int j = 0; j < count; ++j) {
             if (page) page[j] = rows ? own[j] : each ? -2 : -1;
-            c->open(kids[j], len, std::move(tables[j]), stream);
+            c->open(kids[j], len, pages_of(j), stream);
             out[j] = kids[j];
         }
     });
