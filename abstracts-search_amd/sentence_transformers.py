@@ -22,9 +22,11 @@ A model directory in the usual sentence-transformers layout is read directly:
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import json
 import os
+import threading
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 import numpy as np
@@ -84,6 +86,34 @@ def _is_torch(x) -> bool:
 
 
 _DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
+
+class _Prompts(dict):
+    """token ids (a tuple) of each cached prompt -> its handle.  Never changed once made."""
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        # sorted: every prompt that begins as another one stands behind it, with nothing in between that does not; of each, the
+        # longest other one that it begins as
+        self._keys, self._base = sorted(self), []
+        for i, key in enumerate(self._keys):
+            j = i - 1
+            while j >= 0 and key[:len(self._keys[j])] != self._keys[j]:
+                j = self._base[j]
+            self._base.append(j)
+
+    def behind(self, ids):
+        """(length, handle) of the longest prompt that `ids` goes on from, else (0, None)"""
+        if not self:
+            return 0, None
+        ids = tuple(ids)
+        i = bisect.bisect_left(self._keys, ids) - 1
+        while i >= 0:
+            key = self._keys[i]
+            if ids[:len(key)] == key:
+                return len(key), self[key]
+            i = self._base[i]
+        return 0, None
 
 # stella_en_1.5B_v5 (SURVEY Appendix B.1 [PRIOR]; every value is overridable by config.json)
 STELLA_EN_1_5B_V5 = dict(vocab_size=151646, hidden=1536, n_layers=28, n_heads=12, n_kv_heads=2, head_dim=128,
@@ -242,7 +272,8 @@ class SentenceTransformer:
         if causal is not None:
             cfg["causal"] = bool(causal)
         self.config = cfg
-        self._cached_prompts: dict = {}          # token ids of a cached prompt -> its handle
+        self._cached_prompts = _Prompts()        # replaced as a whole, under the lock: an encode keeps to the one it began with
+        self._prompts_lock = threading.Lock()
         c = _Cfg(**{k: (int(v) if isinstance(v, bool) else v) for k, v in cfg.items() if k in dict(_Cfg._fields_)})
         self._h = c_void_p()
         _check(_Lib.get().mi_encoder_create(ctypes.byref(c), self._device_index, ctypes.byref(self._h)))
@@ -326,8 +357,13 @@ class SentenceTransformer:
     def load_weights(self, weights: dict):
         """name -> torch tensor / numpy array (f32, bf16 or f16; host or CUDA)."""
         import torch
+        with self._prompts_lock:                 # (a prompt that another thread caches waits for the new weights)
+            self._drop_prompts()
+            return self._load_weights(weights)
+
+    def _load_weights(self, weights):
+        import torch
         lib = _Lib.get()
-        self._cached_prompts = {}                # (a new weight makes the library drop them)
         for name, t in weights.items():
             if name.startswith("model."):
                 name = name[6:]
@@ -424,27 +460,23 @@ class SentenceTransformer:
         if not ids or len(ids) >= self.max_seq_length:
             raise ValueError(f"cache_prompt: a prompt of 1 .. {self.max_seq_length - 1} tokens, got {len(ids)}")
         key = tuple(ids)
-        if key not in self._cached_prompts:
-            a, n = np.asarray(ids, np.int32), c_int32()
-            stream = c_void_p(torch.cuda.current_stream(torch.device("cuda", self._device_index)).cuda_stream)
-            _check(_Lib.get().mi_encoder_cache_prompt(self._h, len(ids), c_void_p(a.ctypes.data), ctypes.byref(n), stream))
-            self._cached_prompts[key] = n.value
+        with self._prompts_lock:                 # (one thread runs it, the others find it)
+            if key not in self._cached_prompts:
+                a, n = np.asarray(ids, np.int32), c_int32()
+                stream = c_void_p(torch.cuda.current_stream(torch.device("cuda", self._device_index)).cuda_stream)
+                _check(_Lib.get().mi_encoder_cache_prompt(self._h, len(ids), c_void_p(a.ctypes.data), ctypes.byref(n), stream))
+                self._cached_prompts = _Prompts({**self._cached_prompts, key: n.value})
         return len(ids)
 
     def drop_prompts(self) -> None:
         """forgets every cached prompt"""
-        cached, self._cached_prompts = self._cached_prompts, {}
-        for handle in cached.values():
-            _check(_Lib.get().mi_encoder_drop_prompt(self._h, handle))
+        with self._prompts_lock:
+            self._drop_prompts()
 
-    def _behind(self, ids):
-        """(length, handle) of the longest cached prompt that `ids` goes on from, else (0, None)"""
-        best = (0, None)
-        for key, handle in self._cached_prompts.items():
-            n = len(key)
-            if best[0] < n < len(ids) and tuple(ids[:n]) == key:
-                best = (n, handle)
-        return best
+    def _drop_prompts(self):
+        cached, self._cached_prompts = self._cached_prompts, _Prompts()
+        for handle in cached.values():           # (one that the library has dropped by itself is gone all the same)
+            _Lib.get().mi_encoder_drop_prompt(self._h, handle)
 
     # Tokens one forward pass takes: 32 768 = 128 row tiles of 256, with which every GEMM of the stack fills whole
     # rounds of the 256 CUs (N = 1536: 768 tiles = 3.0 rounds, 2048: 4.0, 17 920: 35.0).  sentence-transformers'
@@ -493,44 +525,57 @@ class SentenceTransformer:
         out = torch.empty((n, dim), dtype=torch.float32, device=dev)
         stream = c_void_p(torch.cuda.current_stream(dev).cuda_stream)
         groups = [(None, list(range(n)))]
-        if self._cached_prompts:                 # texts behind the same cached prompt share passes, without its tokens
+        own, cached = token_lists, self._cached_prompts
+        if cached:                               # texts behind the same cached prompt share passes, without its tokens
             by: dict = {}
-            behind = [self._behind(t) for t in token_lists]
+            behind = [cached.behind(t) for t in token_lists]
             for i, (_, handle) in enumerate(behind):
                 by.setdefault(handle, []).append(i)
             few, from_, to = self.prompt_break_even
             for handle, members in list(by.items()):
                 total = sum(len(token_lists[i]) for i in members)
-                own = total - len(members) * behind[members[0]][0]
-                if handle is not None and (total <= few or from_ < own and total <= to):
+                rest = total - len(members) * behind[members[0]][0]
+                if handle is not None and (total <= few or from_ < rest and total <= to):
                     by.setdefault(None, []).extend(by.pop(handle))
                     for i in members:
                         behind[i] = (0, None)
-            token_lists = [t[k:] for t, (k, _) in zip(token_lists, behind)]
+            own = [t[k:] for t, (k, _) in zip(token_lists, behind)]
             groups = list(by.items())
+        gone = []                                # texts whose prompt was dropped meanwhile: with its tokens
         for handle, members in groups:
-            order = sorted(members, key=lambda i: -len(token_lists[i]))
-            self._encode_group(handle, order, token_lists, batch_size, normalize_embeddings, out, stream)
+            gone += self._encode_group(handle, members, own, batch_size, normalize_embeddings, out, stream)
+        if gone:
+            self._encode_group(None, gone, token_lists, batch_size, normalize_embeddings, out, stream)
         if as_tensor:
             return out
         return out.cpu().numpy()
 
-    def _encode_group(self, handle, order, token_lists, batch_size, normalize_embeddings, out, stream):
+    def _encode_group(self, handle, members, token_lists, batch_size, normalize_embeddings, out, stream):
+        """the sequences `members` behind the cached prompt `handle` (None: behind none); those left where there is no such prompt any more"""
         import itertools
-        lib = _Lib.get()
+        lib, gone = _Lib.get(), []
         # every pass only ENQUEUES work (the C ABI stages the token ids through pinned memory and writes embedding i
         # straight to row sel[i] of `out`): the packing of the next pass overlaps the GPU running this one
-        for sel in self._passes(order, token_lists, batch_size):
+        for sel in self._passes(sorted(members, key=lambda i: -len(token_lists[i])), token_lists, batch_size):
             cu = np.zeros(len(sel) + 1, np.int32)
-            np.cumsum([len(token_lists[i]) for i in sel], out=cu[1:])
-            if isinstance(token_lists[sel[0]], np.ndarray):           # id arrays (what `tokenizers` can hand over)
-                ids = np.concatenate([token_lists[i] for i in sel]).astype(np.int32, copy=False)
+            cu[1:] = np.cumsum([len(token_lists[i]) for i in sel])
+            if isinstance(token_lists[sel[0]], np.ndarray):
+                ids = np.concatenate([np.ascontiguousarray(token_lists[i], np.int32) for i in sel])
             else:
                 ids = np.fromiter(itertools.chain.from_iterable(token_lists[i] for i in sel), np.int32, count=int(cu[-1]))
             rows = np.asarray(sel, np.int32)
             args = (len(sel), c_void_p(ids.ctypes.data), c_void_p(cu.ctypes.data), int(normalize_embeddings), c_void_p(out.data_ptr()),
                     c_void_p(rows.ctypes.data), stream)
-            _check(lib.mi_encoder_encode_rows(self._h, *args) if handle is None else lib.mi_encoder_encode_prompted(self._h, handle, *args))
+            if handle is None:
+                _check(lib.mi_encoder_encode_rows(self._h, *args))
+            elif lib.mi_encoder_encode_prompted(self._h, handle, *args):
+                if b"no such cached prompt" not in lib.mi_enc_last_error():
+                    _check(1)
+                gone += sel
+        if gone:
+            with self._prompts_lock:
+                self._cached_prompts = _Prompts({k: h for k, h in self._cached_prompts.items() if h != handle})
+        return gone
 
     # -- parity / measurement hooks ---------------------------------------
     def last_hidden_state(self, token_lists):

@@ -259,3 +259,87 @@ def test_prompts_come_and_go_beside_a_capture(st, tiny):
             model.cache_prompt([1, 2, 3])
         assert c.ended == 0
     assert np.isfinite(model.encode_tokens([[1, 2, 3, 4]])).all()
+
+
+def test_prompts_come_and_go_while_others_encode(st, tiny):
+    """cache_prompt and drop_prompts on one thread, encode_tokens on four: every encode answers, with the prompt's tokens where the prompt
+    has gone meanwhile"""
+    import threading
+    cfg, W = tiny
+    rng = np.random.default_rng(12)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    ids = lambda n: rng.integers(0, cfg.vocab_size, int(n)).tolist()
+    prompts = [ids(n) for n in (5, 30, 64, 100, 150)]
+    prompts += [prompts[3] + ids(20), prompts[1] + ids(1)]
+    work = [[prompts[(i + j) % 7] + ids(rng.integers(1, 60)) for j in range(7)] for i in range(4)]
+    want = [model.encode_tokens(w, normalize_embeddings=True) for w in work]
+    got, errors, stop = [[] for _ in work], [], threading.Event()
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not stop.is_set() or not got[i]:
+                    got[i].append(model.encode_tokens(work[i], normalize_embeddings=True))
+        except Exception as e:                                    # pragma: no cover
+            errors.append(e)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    try:
+        for k in range(40):
+            for p in prompts[k % 3:]:
+                model.cache_prompt(p)
+            for n in range(20):                                   # (many at a time: the table of prompts changes under every lookup)
+                model.cache_prompt([n, k % 50, 1, 2])
+            if k % 2:
+                model.drop_prompts()
+    finally:
+        stop.set()
+        [t.join() for t in ts]
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert g
+        for e in g:
+            same(e, w, 1e-3)
+
+
+def test_two_threads_cache_the_same_prompt(st, tiny):
+    """one of them runs it, and dropping the prompts drops all there are"""
+    import threading
+    cfg, W = tiny
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    p0 = st.debug_counter("prompted_passes")
+    for k in range(10):
+        ts = [threading.Thread(target=model.cache_prompt, args=([k, 1, 2, 3],)) for _ in range(4)]
+        [t.start() for t in ts]
+        [t.join() for t in ts]
+    assert st.debug_counter("prompted_passes") == p0 + 10
+    handles = list(model._cached_prompts.values())
+    model.drop_prompts()
+    assert len(handles) == 10 and not model._cached_prompts
+    for h in handles:
+        assert st._Lib.get().mi_encoder_drop_prompt(model._h, h) != 0
+
+
+def test_a_prompt_the_library_dropped_is_encoded_in_full(st, tiny):
+    cfg, W = tiny
+    rng = np.random.default_rng(2)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    prompt = rng.integers(0, cfg.vocab_size, 80).tolist()
+    toks = [prompt + rng.integers(0, cfg.vocab_size, n).tolist() for n in (3, 40, 9, 1)] + [[4, 5]]
+    plain = model.encode_tokens(toks, normalize_embeddings=True)
+    model.cache_prompt(prompt)
+    st._check(st._Lib.get().mi_encoder_drop_prompt(model._h, next(iter(model._cached_prompts.values()))))
+    for bs in (None, 2):
+        same(model.encode_tokens(toks, normalize_embeddings=True, batch_size=bs), plain, 1e-3)
+    assert not model._cached_prompts
+    model.cache_prompt(prompt)
+    p0 = st.debug_counter("prompted_passes")
+    same(model.encode_tokens(toks, normalize_embeddings=True), plain, 1e-3)
+    assert st.debug_counter("prompted_passes") == p0 + 1
+    model.load_weights({})                                        # (nothing is loaded: the library would have kept them)
+    assert not model._cached_prompts
+    for _ in range(2):                                            # (of 256 prompts)
+        for i in range(200):
+            model.cache_prompt([7, i % 60, i // 60])
+        model.load_weights({})
