@@ -1537,10 +1537,8 @@ int mi_encoder_load_tensor(mi_encoder *h, const char *name_c, const void *data, 
     return guard([&] {
         MI_REQUIRE(h && name_c && data && shape, "null argument");
         MI_REQUIRE(dtype >= 0 && dtype <= 2, "bad dtype");
-        {
-            std::lock_guard<std::mutex> pl(h->prompts_mu);
-            h->prompts.clear();   // any new weight invalidates the cached prompts
-        }
+        std::lock_guard<std::mutex> pl(h->prompts_mu);   // (all along: a prompt that another thread caches sees the whole of the new weight)
+        h->prompts.clear();    // any new weight invalidates the cached prompts
         h->tiled_ok = false;   // .. and the fragment-major copies
         h->few_ok = false;
         h->roped_ok = false;

@@ -343,3 +343,43 @@ def test_a_prompt_the_library_dropped_is_encoded_in_full(st, tiny):
         for i in range(200):
             model.cache_prompt([7, i % 60, i // 60])
         model.load_weights({})
+
+
+def test_a_prompt_cached_while_weights_load_is_of_the_new_ones(st, tiny):
+    """through the C entries: whatever prompt is left when both threads are done gives what its tokens give"""
+    import threading
+    cfg, W = tiny
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    lib, E = st._Lib.get(), torch.from_numpy(np.asarray(W["embed_tokens.weight"], np.float32))
+    E = [E.contiguous(), (E * 1.5).contiguous()]
+    shape = (st.c_int64 * 2)(*E[0].shape)
+    handles, errors = {}, []
+
+    def load():
+        for i in range(60):
+            if lib.mi_encoder_load_tensor(model._h, b"embed_tokens.weight", E[i % 2].data_ptr(), 0, shape, 2):
+                errors.append(lib.mi_enc_last_error())
+
+    t = threading.Thread(target=load)
+    t.start()
+    k = 0
+    while t.is_alive() or k < 5:
+        a, n = np.asarray([1 + k % 50, 2, 3 + k // 50], np.int32), st.c_int32()
+        if lib.mi_encoder_cache_prompt(model._h, 3, a.ctypes.data, st.ctypes.byref(n), None):
+            errors.append(lib.mi_enc_last_error())
+            break
+        handles[n.value] = a.tolist()
+        k += 1
+    t.join()
+    assert not errors, errors
+    left = 0
+    for h, p in handles.items():
+        toks = [p + [9, 4, 7], p + [3]]
+        out, ids = torch.empty(2, 64, device="cuda"), np.asarray([9, 4, 7, 3], np.int32)
+        if lib.mi_encoder_encode_prompted(model._h, h, 2, ids.ctypes.data, np.asarray([0, 3, 4], np.int32).ctypes.data, 1, out.data_ptr(), None, None):
+            assert b"no such cached prompt" in lib.mi_enc_last_error()
+            continue
+        torch.cuda.synchronize()
+        left += 1
+        same(out.cpu().numpy(), model.encode_tokens(toks, normalize_embeddings=True), 1e-3)
+    assert left
