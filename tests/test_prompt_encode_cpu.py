@@ -73,3 +73,43 @@ def test_lookups_beside_prompts_that_come():
     stop.set()
     [t.join() for t in ts]
     assert not errors
+
+
+def groups(texts, prompts, batch_size=None, **attrs):
+    """{prompt's number or None: how many texts} of encode_tokens' passes; texts: [(prompt's number or None, tokens of its own)]"""
+    model = st.SentenceTransformer.__new__(st.SentenceTransformer)
+    for k, v in attrs.items():
+        setattr(model, k, v)
+    keys = [tuple([1000 + i] * n) for i, n in enumerate(prompts)]
+    lists = [list(keys[p] if p is not None else ()) + [7] * own for p, own in texts]
+    run, got = model._groups(lists, st._Prompts({k: i for i, k in enumerate(keys)}), batch_size)
+    assert sorted(i for _, members in got for i in members) == list(range(len(texts)))          # each text once
+    for handle, members in got:
+        for i in members:
+            assert run[i] == (lists[i] if handle is None else lists[i][len(keys[handle]):])
+            assert handle is None or texts[i][0] == handle
+    assert len({h for h, _ in got}) == len(got) and all(m for _, m in got)
+    return {h: len(m) for h, m in got}
+
+
+def test_one_text_behind_each_of_many_prompts_share_a_pass():
+    """a pass a prompt would stream all the weights for each"""
+    assert groups([(i, 5) for i in range(30)], [160] * 30) == {None: 30}
+    assert groups([(i, 5) for i in range(2)], [160] * 2) == {0: 1, 1: 1}
+    many = groups([(i, 60) for i in range(30) for _ in range(8)], [160] * 30)
+    assert many == {i: 8 for i in range(30)}
+    # a prompt with much behind it keeps its pass, the small ones go together, and with the texts behind none
+    assert groups([(0, 50)] * 40 + [(i, 5) for i in range(1, 12)] + [(None, 30)], [400] + [160] * 11) == {0: 40, None: 12}
+    assert groups([(i, 5) for i in range(30)], [160] * 30, prompt_pass_tokens=0) == {i: 1 for i in range(30)}
+    assert groups([(i, 5) for i in range(5)], [4000] * 5) == {i: 1 for i in range(5)}
+    assert groups([], []) == {}
+
+
+def test_short_passes_are_judged_one_by_one():
+    """forty queries of 31 tokens one at a time take the query-time path with their prompt's tokens, as one of them does"""
+    assert groups([(0, 11)], [20]) == {None: 1}
+    assert groups([(0, 11)] * 40, [20], batch_size=1) == {None: 40}
+    assert groups([(0, 11)] * 40, [20]) == {0: 40}
+    assert groups([(0, 11)] * 40, [20], batch_size=1, prompt_break_even=(0, 0, 0)) == {0: 40}
+    assert groups([(0, 11)] * 40, [20], token_budget=None) == {0: 40}
+    assert groups([(0, 29)] * 3, [20], batch_size=1) == {0: 3}

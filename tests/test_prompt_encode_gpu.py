@@ -383,3 +383,21 @@ def test_a_prompt_cached_while_weights_load_is_of_the_new_ones(st, tiny):
         left += 1
         same(out.cpu().numpy(), model.encode_tokens(toks, normalize_embeddings=True), 1e-3)
     assert left
+
+
+@pytest.mark.parametrize("pass_tokens", [0, 1000])
+def test_many_prompts_in_one_call(st, tiny, monkeypatch, pass_tokens):
+    """thirty prompts with a text each: in a pass apiece behind their pages, or together with their tokens; the same either way"""
+    cfg, W = tiny
+    monkeypatch.setattr(st.SentenceTransformer, "prompt_pass_tokens", pass_tokens)
+    rng = np.random.default_rng(21)
+    model = st.SentenceTransformer(config=cfg.to_dict(), weights=W)
+    ids = lambda n: rng.integers(0, cfg.vocab_size, n).tolist()
+    base = ids(100)
+    prompts = [base + ids(60 + i) for i in range(30)]
+    toks = [p + ids(5) for p in prompts] + [prompts[3] + ids(30), ids(12)]
+    for p in prompts:
+        model.cache_prompt(p)
+    p0 = st.debug_counter("prompted_passes")
+    same(model.encode_tokens(toks, normalize_embeddings=True), oracle_encode(cfg, W, toks), 1e-3)
+    assert st.debug_counter("prompted_passes") == p0 + (0 if pass_tokens else 30)
