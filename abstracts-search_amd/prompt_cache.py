@@ -117,13 +117,28 @@ class PromptCache:
         self._close = weakref.finalize(self, _destroy, self._h)
         self._lib = lib
         self._table_cap = -(-max_tokens // PAGE) if max_tokens else n_pages   # pages of the longest entry
-        self._tables: dict = {}                      # entry -> its table, as far as known: a list, or (full pages, the last one)
-        self._moves = 0                              # how often pages have moved
-        self._plans: dict = {}                       # (entry, shapes) -> bytes of workspace, until an entry changes
+        # What is known without asking the library.  Another thread may change it meanwhile: what was learnt before a change carries
+        # the mark of its time, replaced on either side of the change, and is not believed later.
+        self._tables: dict = {}                      # entry -> (full pages, the last one or -1, the mark of moves)
+        self._moves = object()                       # since pages moved last
+        self._plans: dict = {}                       # (entry, shapes, the mark of edits) -> bytes of workspace
+        self._edits = object()                       # since an entry's length changed last
         # torch's current stream as a pointer (building the Stream object first is 1.7 us of a 10 us call)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         index, device = self.device.index, self.device
         self._stream = (lambda: raw(index)) if raw else (lambda: torch.cuda.current_stream(device).cuda_stream)
+
+    def _changed(self, entries) -> None:
+        """lengths change: called on either side of it"""
+        self._edits = object()
+        self._plans.clear()
+        for e in entries:
+            self._tables.pop(e, None)
+
+    def _moved(self) -> None:
+        """page numbers change: called on either side of it"""
+        self._moves = object()
+        self._tables.clear()
 
     # -- prompts ------------------------------------------------------------
     def new(self) -> int:
@@ -134,9 +149,10 @@ class PromptCache:
 
     def reserve(self, entry: int, n: int) -> None:
         """n more tokens at the end of the entry, to be filled by ``write``"""
-        self._plans.clear()
-        self._tables.pop(entry, None)
-        _check(self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream()))
+        self._changed((entry,))
+        rc = self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream())
+        self._changed((entry,))
+        _check(rc)
 
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
         """keys and values of tokens start .. of layers layer ..: [layers, n, n_kv_heads, head_dim], or one layer without the
@@ -151,10 +167,11 @@ class PromptCache:
         k, v = self._kv(k, v)
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
-        self._plans.clear()
-        self._tables.pop(entry, None)
         ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
-        _check(self._lib.mi_prompt_cache_extend(self._h, entry, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs, self._stream()))
+        self._changed((entry,))
+        rc = self._lib.mi_prompt_cache_extend(self._h, entry, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs, self._stream())
+        self._changed((entry,))
+        _check(rc)
 
     def _kv(self, k, v):
         if k.dim() == 3 and v.dim() == 3:
@@ -181,12 +198,10 @@ class PromptCache:
         _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, own, self._stream()))
         kids, own = out[:], own[:]
         if count > 1 and own[0] > -2:                # (their tables without asking for each of them)
-            full = self.table(entry)
+            full = self.table(kids[0])               # (not the parent's: another thread may extend that)
             if own[0] >= 0:
                 full.pop()
-            known = {k: (full, p) for k, p in zip(kids, own)}
-            if moves == self._moves:
-                self._tables.update(known)
+            self._tables.update({k: (full, p, moves) for k, p in zip(kids, own)})
         return kids
 
     def copy(self, entry: int) -> int:
@@ -198,19 +213,18 @@ class PromptCache:
     def free(self, entries) -> None:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
-        self._plans.clear()
-        for e in entries:
-            self._tables.pop(e, None)
-        _check(self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream()))
+        self._changed(entries)
+        rc = self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream())
+        self._changed(())
+        _check(rc)
 
     def compact(self) -> int:
         """moves pages down until the used ones are the first ones of the pool; how many were moved"""
         n = c_int32()
-        self._moves += 1
-        self._tables.clear()
-        _check(self._lib.mi_prompt_cache_compact(self._h, self._stream(), ctypes.byref(n)))
-        self._moves += 1
-        self._tables.clear()
+        self._moved()
+        rc = self._lib.mi_prompt_cache_compact(self._h, self._stream(), ctypes.byref(n))
+        self._moved()
+        _check(rc)
         return n.value
 
     def resize(self, n_pages: int) -> None:
@@ -220,11 +234,10 @@ class PromptCache:
         if n_pages < 1:
             raise ValueError(f"PromptCache.resize: n_pages must be positive, got {n_pages}")
         pages = torch.zeros((n_pages, *self.pages.shape[1:]), dtype=self.dtype, device=self.device)
-        self._moves += 1
-        self._tables.clear()
-        _check(self._lib.mi_prompt_cache_resize(self._h, pages.data_ptr(), n_pages, self._stream()))
-        self._moves += 1
-        self._tables.clear()
+        self._moved()
+        rc = self._lib.mi_prompt_cache_resize(self._h, pages.data_ptr(), n_pages, self._stream())
+        self._moved()
+        _check(rc)
         self.pages = pages
 
     # -- what is held -----------------------------------------------------------
@@ -236,8 +249,8 @@ class PromptCache:
     def table(self, entry: int) -> list[int]:
         """the page numbers of the entry, in order"""
         known = self._tables.get(entry)
-        if known is not None:
-            full, last = known
+        if known is not None and known[2] is self._moves:
+            full, last, _ = known
             return full + [last] if last >= 0 else full[:]
         cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
@@ -312,15 +325,23 @@ class PromptCache:
         qs, os = q.stride(), out.stride()
         head = (entry, layer, heads, tokens, keys, texts, q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                 cq, ck, causal, scale, rest, 0)
-        shape = (entry, heads, tokens, keys, texts)
+        shape = (entry, heads, tokens, keys, texts, self._edits)
         need = self._plans.get(shape)
         if need is None:
-            n = c_int64()
-            _check(self._lib.mi_prompt_attention_workspace(self._h, _ATTN.pack(*head, 0, 0), ctypes.byref(n)))
-            need = n.value
+            need = self._workspace(head)
             if len(self._plans) > 1000:
                 self._plans.clear()
             self._plans[shape] = need
-        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-        _check(self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need else 0, need), self._stream()))
-        return out
+        while True:
+            ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+            if not self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need else 0, need), self._stream()):
+                return out
+            why, had = self._lib.mi_enc_last_error().decode(), need
+            need = self._workspace(head)
+            if need <= had:                          # (else another thread has made the prompt longer in between)
+                raise RuntimeError("mi_prompt_cache: " + why)
+
+    def _workspace(self, head) -> int:
+        n = c_int64()
+        _check(self._lib.mi_prompt_attention_workspace(self._h, _ATTN.pack(*head, 0, 0), ctypes.byref(n)))
+        return n.value

@@ -880,3 +880,74 @@ def test_an_infinity_among_the_own_values(pc, dtype, prompt, lens, past):
             sees[max(0, cu_q[1] - back):cu_q[1], 4:, 5] = True
             assert (out[sees] == what).all(), (what, back)
             close(out[~sees], o[~sees], b[~sees])
+
+
+class Between:
+    """the library, with `what()` called once before or behind a function: another thread's call in that place"""
+
+    def __init__(self, cache, name, what, before=False):
+        self.lib, self.name, self.what, self.before = cache._lib, name, what, before
+
+    def __getattr__(self, name):
+        f = getattr(self.lib, name)
+        if name != self.name or self.what is None:
+            return f
+
+        def call(*a):
+            what, self.what = self.what, None
+            if self.before:
+                what()
+            rc = f(*a)
+            if not self.before:
+                what()
+            return rc
+        return call
+
+
+def test_a_prompt_that_grows_between_two_calls_of_one_attention(pc):
+    """the workspace is asked for, another thread extends the entry: the attention of the longer prompt needs more of it, now and in
+    the calls that follow"""
+    _, _, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 8, 2, 128, 200, [2, 1])
+    cache = pc.PromptCache(2, 2, 128, 200)
+    e = cache.new()
+    cache.extend(e, pk.expand(2, -1, -1, -1), pv.expand(2, -1, -1, -1))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k2, v2 = (torch.randn(2, 9000, 2, 128, generator=g, device="cuda").to(BF) for _ in range(2))
+    cache._lib = Between(cache, "mi_prompt_attention_workspace", lambda: cache.extend(e, k2, v2))
+    o, b = reference_many(q, torch.cat([pk, k2[1]]), torch.cat([pv, v2[1]]), k, v, cu_q, cu_k, True)
+    for _ in range(3):
+        close(cache.attention(e, 1, q, k, v, dev(cu_q), dev(cu_k)), o, b)
+
+
+def test_forks_of_a_parent_that_grows_and_of_pages_that_move(pc):
+    """the forks' tables are the forks', whatever another thread does to the parent or the pool before fork comes back"""
+    for length in (64, 100, 200):
+        cache = pc.PromptCache(1, 1, 64, 40)
+        kv = torch.randn(1, 300, 1, 64, device="cuda").to(BF)
+        low, e = cache.new(), cache.new()
+        cache.extend(low, kv[:, :70], kv[:, :70])
+        cache.extend(e, kv[:, :length], kv[:, :length])
+
+        def ask(x):                                           # the library's own answer
+            t, n = (pc.c_int32 * 40)(), pc.c_int32()
+            pc._check(pc._Lib.get().mi_prompt_cache_entry(cache._h, x, pc.ctypes.byref(n), t, 40))
+            return t[:-(-n.value // 64)]
+
+        cache._lib = Between(cache, "mi_prompt_cache_entry", lambda: cache.extend(e, kv, kv), before=True)
+        kids = cache.fork(e, 3)
+        assert [cache.table(x) for x in kids] == [ask(x) for x in kids]
+        assert [cache.length(x) for x in kids] == [length] * 3
+        cache._lib = Between(cache, "mi_prompt_cache_fork", lambda: (cache.free(low), cache.compact()))
+        kids += cache.fork(kids[0], 2)
+        assert [cache.table(x) for x in kids] == [ask(x) for x in kids]
+
+        class Late(dict):                                     # .. and where the move comes just before the tables are noted
+            def update(self, known):
+                cache.free(kids[1])
+                cache.compact()
+                super().update(known)
+
+        cache._tables = Late(cache._tables)
+        kids += cache.fork(kids[0], 2)
+        del kids[1]
+        assert [cache.table(x) for x in kids] == [ask(x) for x in kids]
