@@ -287,8 +287,10 @@ class PromptCache:
             raise ValueError("PromptCache.attention: k and v come together")
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))):
             raise ValueError("PromptCache.attention has no gradient: call it under torch.no_grad()")
-        if q.dtype != dtype or q.device != device or not q.is_contiguous() or q.data_ptr() & 15:
+        qs = q.stride()                              # (is_contiguous() does not look at the strides of axes of length 1)
+        if q.dtype != dtype or q.device != device or qs[2] != 1 or (qs[0] | qs[1]) & 7 or q.data_ptr() & 15:
             q = self._fit(q, "q")
+            qs = q.stride()
         tokens, heads, _ = q.shape
         if k is None:
             keys, kp, vp, ks, vs = 0, 0, 0, (0, 0), (0, 0)
@@ -315,14 +317,18 @@ class PromptCache:
         rest = out is None
         if rest:
             out = q.new_empty((tokens, heads, hd))
-        elif (out.dtype != dtype or out.device != device or out.shape != q.shape or out.stride(2) != 1 or out.data_ptr() & 15
-              or out.stride(0) & 7 or out.stride(1) & 7):
-            raise ValueError(f"PromptCache.attention: out {tuple(q.shape)} {dtype} on {device} with 16-byte aligned rows")
+            os = (heads * hd, hd)
+        else:
+            if out.dtype != dtype or out.device != device or out.shape != q.shape:
+                raise ValueError(f"PromptCache.attention: out {tuple(q.shape)} {dtype} on {device}, got {tuple(out.shape)} {out.dtype} on {out.device}")
+            os = out.stride()
+            os = (os[0] if tokens > 1 else 0, os[1] if heads > 1 else 0, os[2])
+            if os[2] != 1 or (os[0] | os[1]) & 7 or out.data_ptr() & 15:
+                raise ValueError(f"PromptCache.attention: out with 16-byte aligned rows, got strides {out.stride()}")
         if scale is None:
             scale = hd ** -0.5
         elif not 0 <= scale < math.inf:
             raise ValueError(f"PromptCache.attention: scale must be finite and not negative, got {scale}")
-        qs, os = q.stride(), out.stride()
         head = (entry, layer, heads, tokens, keys, texts, q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                 cq, ck, causal, scale, rest, 0)
         shape = (entry, heads, tokens, keys, texts, self._edits)

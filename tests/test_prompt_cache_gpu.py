@@ -951,3 +951,19 @@ def test_forks_of_a_parent_that_grows_and_of_pages_that_move(pc):
         kids += cache.fork(kids[0], 2)
         del kids[1]
         assert [cache.table(x) for x in kids] == [ask(x) for x in kids]
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 6), (1, 1), (5, 1), (2, 6)])
+def test_axes_of_length_one_with_odd_strides(pc, tokens, heads):
+    """one token, or one head, cut from a padded buffer: a stride that nothing is reached by may be anything"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, heads, 1, 64, 70, [tokens])
+    odd = lambda t: torch.nn.functional.pad(torch.cat([t, t]).flatten(1), (0, 4))[:, :t[0].numel()].unflatten(1, t.shape[1:])[:len(t)]
+    one = lambda t: t.contiguous().as_strided(t.shape, (t.stride(0), 5, 1)) if t.shape[1] == 1 else t
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    for cut in (odd, one):
+        q1, k1, v1 = cut(q), cut(k), cut(v)
+        assert torch.equal(q1, q) and (cut is one or q1.stride(0) % 8)
+        close(cache.attention(e, 1, q1, k1, v1), o, b)
+        out = one(torch.zeros_like(q)) if tokens > 1 else odd(torch.zeros_like(q))
+        assert cache.attention(e, 1, q1, k1, v1, out=out) is out
+        close(out, o, b)
