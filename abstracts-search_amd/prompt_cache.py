@@ -325,6 +325,8 @@ class PromptCache:
             os = (os[0] if tokens > 1 else 0, os[1] if heads > 1 else 0, os[2])
             if os[2] != 1 or (os[0] | os[1]) & 7 or out.data_ptr() & 15:
                 raise ValueError(f"PromptCache.attention: out with 16-byte aligned rows, got strides {out.stride()}")
+            if tokens > 1 and os[0] == 0 or heads > 1 and os[1] == 0:
+                raise ValueError("PromptCache.attention: out is broadcast: several of its rows are the same memory")
         if scale is None:
             scale = hd ** -0.5
         elif not 0 <= scale < math.inf:

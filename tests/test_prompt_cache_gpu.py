@@ -967,3 +967,14 @@ def test_axes_of_length_one_with_odd_strides(pc, tokens, heads):
         out = one(torch.zeros_like(q)) if tokens > 1 else odd(torch.zeros_like(q))
         assert cache.attention(e, 1, q1, k1, v1, out=out) is out
         close(out, o, b)
+
+
+def test_an_output_that_is_broadcast_is_refused(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [3])
+    for out in (torch.zeros_like(q[:1]).expand(3, -1, -1), torch.zeros_like(q[:, :1]).expand(-1, 4, -1)):
+        with pytest.raises(ValueError, match="broadcast"):
+            cache.attention(e, 1, q, k, v, out=out)
+    one = torch.zeros_like(q[:1, :1]).expand(1, 1, 64)
+    cache2, e2, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 1, 1, 64, 70, [1])
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    close(cache2.attention(e2, 1, q, k, v, out=one), o, b)
