@@ -117,28 +117,14 @@ class PromptCache:
         self._close = weakref.finalize(self, _destroy, self._h)
         self._lib = lib
         self._table_cap = -(-max_tokens // PAGE) if max_tokens else n_pages   # pages of the longest entry
-        # What is known without asking the library.  Another thread may change it meanwhile: what was learnt before a change carries
-        # the mark of its time, replaced on either side of the change, and is not believed later.
-        self._tables: dict = {}                      # entry -> (full pages, the last one or -1, the mark of moves)
-        self._moves = object()                       # since pages moved last
-        self._plans: dict = {}                       # (entry, shapes, the mark of edits) -> bytes of workspace
-        self._edits = object()                       # since an entry's length changed last
+        # What is known without asking the library.  Another thread may change it meanwhile: either dict is replaced on both sides of
+        # a change, and what was learnt before it goes into the one that was there then.
+        self._tables: dict = {}                      # entry -> its table, as far as known: (full pages, the last one or -1), until pages move
+        self._plans: dict = {}                       # (entry, shapes) -> bytes of workspace, until an entry's length changes
         # torch's current stream as a pointer (building the Stream object first is 1.7 us of a 10 us call)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         index, device = self.device.index, self.device
         self._stream = (lambda: raw(index)) if raw else (lambda: torch.cuda.current_stream(device).cuda_stream)
-
-    def _changed(self, entries) -> None:
-        """lengths change: called on either side of it"""
-        self._edits = object()
-        self._plans.clear()
-        for e in entries:
-            self._tables.pop(e, None)
-
-    def _moved(self) -> None:
-        """page numbers change: called on either side of it"""
-        self._moves = object()
-        self._tables.clear()
 
     # -- prompts ------------------------------------------------------------
     def new(self) -> int:
@@ -149,9 +135,10 @@ class PromptCache:
 
     def reserve(self, entry: int, n: int) -> None:
         """n more tokens at the end of the entry, to be filled by ``write``"""
-        self._changed((entry,))
+        self._plans = {}
+        self._tables.pop(entry, None)
         rc = self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream())
-        self._changed((entry,))
+        self._plans = {}
         _check(rc)
 
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
@@ -163,14 +150,15 @@ class PromptCache:
                                                self._stream()))
 
     def extend(self, entry: int, k, v) -> None:
-        """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim]"""
+        """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim]."""
         k, v = self._kv(k, v)
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
         ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
-        self._changed((entry,))
+        self._plans = {}
+        self._tables.pop(entry, None)
         rc = self._lib.mi_prompt_cache_extend(self._h, entry, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs, self._stream())
-        self._changed((entry,))
+        self._plans = {}
         _check(rc)
 
     def _kv(self, k, v):
@@ -194,14 +182,14 @@ class PromptCache:
         a captured `write` reaches) copied"""
         if count < 0:
             raise ValueError(f"PromptCache.fork: count must not be negative, got {count}")
-        out, own, moves = (c_int32 * count)(), (c_int32 * count)(), self._moves
+        out, own, tables = (c_int32 * count)(), (c_int32 * count)(), self._tables
         _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, own, self._stream()))
         kids, own = out[:], own[:]
         if count > 1 and own[0] > -2:                # (their tables without asking for each of them)
             full = self.table(kids[0])               # (not the parent's: another thread may extend that)
             if own[0] >= 0:
                 full.pop()
-            self._tables.update({k: (full, p, moves) for k, p in zip(kids, own)})
+            tables.update({k: (full, p) for k, p in zip(kids, own)})
         return kids
 
     def copy(self, entry: int) -> int:
@@ -213,17 +201,19 @@ class PromptCache:
     def free(self, entries) -> None:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
-        self._changed(entries)
+        self._plans = {}
+        for e in entries:
+            self._tables.pop(e, None)
         rc = self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream())
-        self._changed(())
+        self._plans = {}
         _check(rc)
 
     def compact(self) -> int:
         """moves pages down until the used ones are the first ones of the pool; how many were moved"""
         n = c_int32()
-        self._moved()
+        self._tables = {}
         rc = self._lib.mi_prompt_cache_compact(self._h, self._stream(), ctypes.byref(n))
-        self._moved()
+        self._tables = {}
         _check(rc)
         return n.value
 
@@ -234,9 +224,9 @@ class PromptCache:
         if n_pages < 1:
             raise ValueError(f"PromptCache.resize: n_pages must be positive, got {n_pages}")
         pages = torch.zeros((n_pages, *self.pages.shape[1:]), dtype=self.dtype, device=self.device)
-        self._moved()
+        self._tables = {}
         rc = self._lib.mi_prompt_cache_resize(self._h, pages.data_ptr(), n_pages, self._stream())
-        self._moved()
+        self._tables = {}
         _check(rc)
         self.pages = pages
 
@@ -249,8 +239,8 @@ class PromptCache:
     def table(self, entry: int) -> list[int]:
         """the page numbers of the entry, in order"""
         known = self._tables.get(entry)
-        if known is not None and known[2] is self._moves:
-            full, last, _ = known
+        if known is not None:
+            full, last = known
             return full + [last] if last >= 0 else full[:]
         cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
@@ -333,13 +323,13 @@ class PromptCache:
             raise ValueError(f"PromptCache.attention: scale must be finite and not negative, got {scale}")
         head = (entry, layer, heads, tokens, keys, texts, q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                 cq, ck, causal, scale, rest, 0)
-        shape = (entry, heads, tokens, keys, texts, self._edits)
-        need = self._plans.get(shape)
+        shape, plans = (entry, heads, tokens, keys, texts), self._plans
+        need = plans.get(shape)
         if need is None:
             need = self._workspace(head)
-            if len(self._plans) > 1000:
-                self._plans.clear()
-            self._plans[shape] = need
+            if len(plans) > 1000:
+                plans.clear()
+            plans[shape] = need
         while True:
             ws = q.new_empty((need,), dtype=torch.uint8) if need else None
             if not self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need else 0, need), self._stream()):
