@@ -75,6 +75,18 @@ def _check(rc: int):
         raise RuntimeError("mi_prompt_cache: " + _Lib.get().mi_enc_last_error().decode())
 
 
+def _no_gradient(what, *tensors):
+    """refuses tensors whose gradient (of either mode) would be lost"""
+    import torch
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"PromptCache.{what} has no gradient: call it under torch.no_grad()")
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and any(t is not None and forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"PromptCache.{what} has no gradient: a tensor carries a forward-mode tangent")
+
+
 def _destroy(handle):
     try:
         _Lib.get().mi_prompt_cache_destroy(handle)
@@ -143,15 +155,15 @@ class PromptCache:
 
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
         """keys and values of tokens start .. of layers layer ..: [layers, n, n_kv_heads, head_dim], or one layer without the
-        first axis.  Tokens in pages that other entries share are refused."""
-        k, v = self._kv(k, v)
+        first axis.  Tokens in pages that other entries share are refused.  No gradient."""
+        k, v = self._kv(k, v, "write")
         ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
         _check(self._lib.mi_prompt_cache_write(self._h, entry, layer, k.shape[0], start, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs,
                                                self._stream()))
 
     def extend(self, entry: int, k, v) -> None:
-        """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim]."""
-        k, v = self._kv(k, v)
+        """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim].  No gradient."""
+        k, v = self._kv(k, v, "extend")
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
         ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
@@ -161,7 +173,8 @@ class PromptCache:
         self._plans = {}
         _check(rc)
 
-    def _kv(self, k, v):
+    def _kv(self, k, v, what):
+        _no_gradient(what, k, v)
         if k.dim() == 3 and v.dim() == 3:
             k, v = k[None], v[None]
         want = (self.n_kv_heads, self.head_dim)
@@ -275,8 +288,9 @@ class PromptCache:
             raise ValueError(f"PromptCache.attention: q [tokens, heads, {hd}], got {tuple(q.shape)}")
         if (k is None) != (v is None):
             raise ValueError("PromptCache.attention: k and v come together")
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))):
-            raise ValueError("PromptCache.attention has no gradient: call it under torch.no_grad()")
+        if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad)) or (out is not None and out.requires_grad))
+                or getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0):
+            _no_gradient("attention", q, k, v, out)
         qs = q.stride()                              # (is_contiguous() does not look at the strides of axes of length 1)
         if q.dtype != dtype or q.device != device or qs[2] != 1 or (qs[0] | qs[1]) & 7 or q.data_ptr() & 15:
             q = self._fit(q, "q")
@@ -333,6 +347,8 @@ class PromptCache:
         while True:
             ws = q.new_empty((need,), dtype=torch.uint8) if need else None
             if not self._lib.mi_prompt_attention(self._h, _ATTN.pack(*head, ws.data_ptr() if need else 0, need), self._stream()):
+                if not rest:
+                    torch.autograd.graph.increment_version(out)    # (a backward pass that saved it has to notice)
                 return out
             why, had = self._lib.mi_enc_last_error().decode(), need
             need = self._workspace(head)

@@ -978,3 +978,38 @@ def test_an_output_that_is_broadcast_is_refused(pc):
     cache2, e2, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 1, 1, 64, 70, [1])
     o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
     close(cache2.attention(e2, 1, q, k, v, out=one), o, b)
+
+
+def test_gradients_are_refused_not_lost(pc):
+    """tensors that need one, forward-mode tangents, and an output that a backward pass has saved"""
+    import torch.autograd.forward_ad as forward
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [3])
+    want = cache.attention(e, 1, q, k, v)
+    t = torch.randn(2, 5, 2, 64, device="cuda").to(BF)
+    leaf = lambda x: x.clone().requires_grad_()
+    for f in (lambda: cache.extend(e, leaf(t), t), lambda: cache.extend(e, t, leaf(t)), lambda: cache.write(e, leaf(t), t, 65), lambda: cache.write(e, t, leaf(t) * 2, 65),
+              lambda: cache.attention(e, 1, leaf(q), k, v), lambda: cache.attention(e, 1, q, leaf(k), v), lambda: cache.attention(e, 1, q, k, leaf(v)),
+              lambda: cache.attention(e, 1, q, k, v, out=leaf(q)), lambda: torch.func.vjp(lambda x: cache.attention(e, 1, x, k, v), q)):
+        with pytest.raises(ValueError, match="gradient"):
+            f()
+    with torch.no_grad(), forward.dual_level():
+        dual = lambda x: forward.make_dual(x, torch.ones_like(x))
+        for f in (lambda: cache.extend(e, dual(t), t), lambda: cache.write(e, t, dual(t), 65), lambda: cache.attention(e, 1, dual(q), k, v),
+                  lambda: cache.attention(e, 1, q, k, dual(v))):
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+        assert torch.equal(cache.attention(e, 1, q, k, v), want)
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda x: cache.attention(e, 1, x, k, v), (q,), (q,))
+    assert cache.length(e) == 70
+    out, w = torch.zeros_like(q), leaf(q)
+    loss = (out * w).sum()
+    cache.attention(e, 1, q, k, v, out=out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(cache.attention(e, 1, leaf(q), k, v, out=torch.empty_like(q)), want)
+    with torch.no_grad():
+        cache.extend(e, leaf(t), t)
+    assert cache.length(e) == 75
