@@ -21,6 +21,9 @@ void *const ANY = reinterpret_cast<void *>(~uintptr_t(0));
 // .. and for work of several streams: equal to none, so that whoever takes the page waits for the device
 void *const SEVERAL = reinterpret_cast<void *>(~uintptr_t(1));
 
+// work on a is in order with work on b (the per-thread handle is another stream in every thread)
+bool same(void *a, void *b) { return a == b && a != reinterpret_cast<void *>(hipStreamPerThread); }
+
 bool capturing(void *stream) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     MI_HIP(hipStreamIsCapturing(as_stream(stream), &st));
@@ -90,12 +93,12 @@ struct mi_prompt_cache {
         got.reserve(n);
         if (n) free_pages.each([&](int32_t p) { got.push_back(p); return (int)got.size() < n; });
         for (int32_t p : got)
-            if (tag[p] != ANY && tag[p] != stream) { wait_all(); break; }
+            if (tag[p] != ANY && !same(tag[p], stream)) { wait_all(); break; }
         return got;
     }
     void take(int32_t p) { free_pages.erase(p); ref[p] = 1; tag[p] = ANY; }
     void drop(int32_t p, void *stream) {
-        if (stream != ANY) tag[p] = tag[p] == ANY || tag[p] == stream ? stream : SEVERAL;
+        if (stream != ANY) tag[p] = tag[p] == ANY || same(tag[p], stream) ? stream : SEVERAL;
         if (--ref[p] == 0) free_pages.insert(p);
     }
     std::vector<int32_t> pick_entries(int n, void *stream) {
@@ -104,7 +107,7 @@ struct mi_prompt_cache {
             if (!entries[e].live) got.push_back(e);
         if ((int)got.size() != n) throw Error("prompt cache: more than max_entries (" + std::to_string(cfg.max_entries) + ") entries");
         for (int32_t e : got)
-            if (entries[e].slot_tag != ANY && entries[e].slot_tag != stream) { wait_all(); break; }
+            if (entries[e].slot_tag != ANY && !same(entries[e].slot_tag, stream)) { wait_all(); break; }
         return got;
     }
     void open(int32_t e, int len, std::vector<int32_t> pg, void *stream) {
@@ -112,7 +115,7 @@ struct mi_prompt_cache {
         x.live = true; x.len = len; x.pages = std::move(pg); x.home = stream; x.foreign = false; x.graph_from = INT32_MAX; x.slot_tag = ANY;
     }
     void reads(Entry &e, void *stream, bool cap) {
-        if (cap || stream != e.home) e.foreign = true;
+        if (cap || !same(stream, e.home)) e.foreign = true;
     }
     // src[j] -> dst[j]; into: the new entry that the pages dst make up; kids, parent: the new entries that fork `parent`; move: the pages
     // leave src, whose numbers in all tables become dst's (ascending, and no page goes up: a word that one launch of the list has
@@ -128,7 +131,7 @@ struct mi_prompt_cache {
         const int have = (int)e.pages.size(), need = (int)(((int64_t)e.len + n + PC_PAGE - 1) / PC_PAGE);
         if (need <= have) return {};
         std::vector<int32_t> got = pick_pages(need - have, stream);
-        if (stream != e.home) {          // (its table may be in use on the home stream)
+        if (!same(stream, e.home)) {     // (its table may be in use on the home stream)
             wait_all();
             e.foreign = true;
         }
@@ -210,7 +213,7 @@ void write_args(mi_prompt_cache *c, int32_t entry, int32_t layer, int32_t n_laye
     for (int p = start / PC_PAGE; p < (start + n + PC_PAGE - 1) / PC_PAGE; ++p) {
         MI_REQUIRE(c->ref[e.pages[p]] == 1, "prompt cache: tokens in a page that other entries share cannot be written");
         void *const t = c->tag[e.pages[p]];
-        wait = wait || (t != ANY && (t != stream || cap));         // (a replay may run on any stream)
+        wait = wait || (t != ANY && (!same(t, stream) || cap));         // (a replay may run on any stream)
     }
     if (wait) c->wait_all();
     if (cap && n) e.graph_from = std::min(e.graph_from, start / PC_PAGE);
@@ -547,7 +550,7 @@ int mi_prompt_cache_free(mi_prompt_cache *c, int32_t n, const int32_t *list, voi
             const Entry &e = c->at(list[i]);
             if (seen[list[i]]) throw Error("prompt cache: an entry is freed twice");
             seen[list[i]] = true;
-            wait = wait || e.foreign || e.home != stream;
+            wait = wait || e.foreign || !same(e.home, stream);
         }
         if (wait) c->wait_all();
         void *const tag = wait ? ANY : stream;
@@ -579,9 +582,9 @@ int mi_prompt_cache_compact(mi_prompt_cache *c, void *stream, int32_t *moved) {
         if (moved) *moved = (int32_t)src.size();
         if (src.empty()) return;
         bool cross = false;
-        for (const Entry &e : c->entries) cross = cross || (e.live && (e.foreign || e.home != stream));
+        for (const Entry &e : c->entries) cross = cross || (e.live && (e.foreign || !same(e.home, stream)));
         for (const std::vector<int32_t> *pages : {&dst, &src})
-            for (int32_t p : *pages) cross = cross || (c->tag[p] != ANY && c->tag[p] != stream);
+            for (int32_t p : *pages) cross = cross || (c->tag[p] != ANY && !same(c->tag[p], stream));
         if (cross) c->wait_all();
         c->copy_pages(c->pages, c->pages, src.data(), dst.data(), (int)src.size(), PC_PAGE, as_stream(stream), -1, nullptr, -1, 0, true);
         std::vector<int32_t> to(n);

@@ -139,6 +139,8 @@ int mi_enc_gemm_bf16(int device, int M, int N, int K, const void *A, const void 
  * reads, are given out again only after the device has been waited for.  mi_prompt_attention and mi_prompt_cache_write may be
  * captured into a graph (a replay uses the entry's length as it was at the capture; the entry must live, page moves by
  * mi_prompt_cache_compact are followed, a resize ends its use); the other calls are refused on a stream that is being captured.
+ * A stream that entries were made or freed on must have finished its work when it is destroyed; on the per-thread handle, which is another
+ * stream in every thread, whatever is handed on is waited for.
  * A capture that another thread has open is left alone: no call here fails because of it or ends it, also where it waits.
  * ------------------------------------------------------------------------------------------------------------------- */
 #define MI_PROMPT_PAGE 64
@@ -155,7 +157,7 @@ typedef struct mi_prompt_cache_cfg {
     int32_t max_tokens;    /* of one entry (0: all the pages hold) */
 } mi_prompt_cache_cfg;
 
-/* pages: device memory of the caller for the pool, 16-byte aligned, kept until destroy / move; NULL: the cache allocates it. */
+/* pages: device memory of the caller for the pool, 16-byte aligned, kept until destroy or resize; NULL: the cache allocates it. */
 int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pages, mi_prompt_cache **out);
 int mi_prompt_cache_destroy(mi_prompt_cache *c);
 

@@ -1013,3 +1013,43 @@ def test_gradients_are_refused_not_lost(pc):
     with torch.no_grad():
         cache.extend(e, leaf(t), t)
     assert cache.length(e) == 75
+
+
+def test_the_per_thread_stream_is_another_one_in_every_thread(pc):
+    """a page that one thread gives up on its per-thread stream, where it is still read, and another takes on its own: the same
+    handle, not the same stream"""
+    import threading
+    cache = pc.PromptCache(1, 1, 64, 1, max_entries=1)
+    kv, q = torch.randn(1, 64, 1, 64, device="cuda", dtype=BF), torch.randn(1, 2, 64, device="cuda", dtype=BF)
+    nothing, out, steps, done = kv * 0, torch.empty_like(q), [], [threading.Event(), threading.Event()]
+    e = cache.new()
+    cache.extend(e, kv, kv)
+    want = cache.attention(e, 0, q)
+    cache.free(e)
+    torch.cuda.synchronize()
+
+    def first():
+        with torch.cuda.stream(torch.cuda.ExternalStream(2)):     # hipStreamPerThread
+            x = cache.new()
+            cache.extend(x, kv, kv)
+            torch.cuda._sleep(20_000_000)
+            cache.attention(x, 0, q, out=out)
+            cache.free(x)
+            steps.append(torch.cuda.Event())
+            steps[0].record()
+        done[0].set()
+        done[1].wait(60)                                      # (the thread and its stream live until the other is done)
+
+    def second():
+        done[0].wait(60)
+        with torch.cuda.stream(torch.cuda.ExternalStream(2)):
+            x = cache.new()
+            cache.extend(x, nothing, nothing)
+            steps.append(steps[0].query())
+        done[1].set()
+
+    ts = [threading.Thread(target=f) for f in (first, second)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    torch.cuda.synchronize()
+    assert steps[1] is True and torch.equal(out, want) and (cache.pages == 0).all()
