@@ -237,6 +237,7 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     MI_REQUIRE(x.n_heads > 0 && x.n_heads % g.n_kv_heads == 0, "prompt attention: n_heads must be a multiple of the cache's n_kv_heads");
     MI_REQUIRE(x.n_tokens >= 0 && x.n_keys >= 0 && x.n_texts >= 1, "prompt attention: negative count, or no text");
     MI_REQUIRE(x.n_tokens <= 0x7fffff00 / x.n_heads, "prompt attention: more than 2^31 rows");
+    MI_REQUIRE(x.n_keys <= 0x7fffff00, "prompt attention: more than 2^31 keys");   // (a chunk's end stays an int)
     MI_REQUIRE(!x.n_tokens || (x.q && x.out), "null argument");
     MI_REQUIRE(!x.n_keys || (x.k && x.v), "null argument");
     MI_REQUIRE((x.cu_q != nullptr) == (x.cu_k != nullptr), "prompt attention: cu_q and cu_k come together");

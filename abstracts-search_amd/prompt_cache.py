@@ -75,6 +75,13 @@ def _check(rc: int):
         raise RuntimeError("mi_prompt_cache: " + _Lib.get().mi_enc_last_error().decode())
 
 
+def _int32(what, *numbers):
+    """refuses what ctypes would cut to 32 bits"""
+    for n in numbers:
+        if not -1 << 31 <= n < 1 << 31:
+            raise ValueError(f"PromptCache.{what}: {n} is no int32")
+
+
 def _no_gradient(what, *tensors):
     """refuses tensors whose gradient (of either mode) would be lost"""
     import torch
@@ -110,10 +117,10 @@ class PromptCache:
         if head_dim not in (64, 128):
             raise ValueError(f"PromptCache: head_dim must be 64 or 128, got {head_dim}")
         for name, n in (("n_layers", n_layers), ("n_kv_heads", n_kv_heads), ("n_pages", n_pages), ("max_entries", max_entries)):
-            if n < 1:
-                raise ValueError(f"PromptCache: {name} must be positive, got {n}")
-        if max_tokens is not None and max_tokens < 1:
-            raise ValueError(f"PromptCache: max_tokens must be positive, got {max_tokens}")
+            if not 1 <= n < 1 << 31:
+                raise ValueError(f"PromptCache: {name} must be positive (and an int32), got {n}")
+        if max_tokens is not None and not 1 <= max_tokens < 1 << 31:
+            raise ValueError(f"PromptCache: max_tokens must be positive (and an int32), got {max_tokens}")
         lib = _Lib.get()
         if not torch.cuda.is_available():
             raise RuntimeError("mi_prompt_cache: no HIP device available: the MI355X prompt cache has no CPU fallback")
@@ -128,6 +135,7 @@ class PromptCache:
         _check(lib.mi_prompt_cache_create(ctypes.byref(cfg), self.device.index, self.pages.data_ptr(), ctypes.byref(self._h)))
         self._close = weakref.finalize(self, _destroy, self._h)
         self._lib = lib
+        self._max_entries = max_entries
         self._table_cap = -(-max_tokens // PAGE) if max_tokens else n_pages   # pages of the longest entry
         # What is known without asking the library.  Another thread may change it meanwhile: either dict is replaced on both sides of
         # a change, and what was learnt before it goes into the one that was there then.
@@ -147,6 +155,7 @@ class PromptCache:
 
     def reserve(self, entry: int, n: int) -> None:
         """n more tokens at the end of the entry, to be filled by ``write``"""
+        _int32("reserve", entry, n)
         self._plans = {}
         self._tables.pop(entry, None)
         rc = self._lib.mi_prompt_cache_reserve(self._h, entry, n, self._stream())
@@ -156,6 +165,7 @@ class PromptCache:
     def write(self, entry: int, k, v, start: int, layer: int = 0) -> None:
         """keys and values of tokens start .. of layers layer ..: [layers, n, n_kv_heads, head_dim], or one layer without the
         first axis.  Tokens in pages that other entries share are refused.  No gradient."""
+        _int32("write", entry, start, layer)
         k, v = self._kv(k, v, "write")
         ks, vs = _Strides(*k.stride()[:3]), _Strides(*v.stride()[:3])
         _check(self._lib.mi_prompt_cache_write(self._h, entry, layer, k.shape[0], start, k.shape[1], k.data_ptr(), ks, v.data_ptr(), vs,
@@ -163,6 +173,7 @@ class PromptCache:
 
     def extend(self, entry: int, k, v) -> None:
         """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim].  No gradient."""
+        _int32("extend", entry)
         k, v = self._kv(k, v, "extend")
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
@@ -195,6 +206,9 @@ class PromptCache:
         a captured `write` reaches) copied"""
         if count < 0:
             raise ValueError(f"PromptCache.fork: count must not be negative, got {count}")
+        _int32("fork", entry)
+        if count > self._max_entries:
+            raise RuntimeError(f"mi_prompt_cache: prompt cache: more than max_entries ({self._max_entries}) entries")
         out, own, tables = (c_int32 * count)(), (c_int32 * count)(), self._tables
         _check(self._lib.mi_prompt_cache_fork(self._h, entry, count, out, own, self._stream()))
         kids, own = out[:], own[:]
@@ -207,6 +221,7 @@ class PromptCache:
 
     def copy(self, entry: int) -> int:
         """a new entry with the same tokens in pages of its own"""
+        _int32("copy", entry)
         e = c_int32()
         _check(self._lib.mi_prompt_cache_copy(self._h, entry, ctypes.byref(e), self._stream()))
         return e.value
@@ -214,6 +229,7 @@ class PromptCache:
     def free(self, entries) -> None:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
+        _int32("free", *entries)
         self._plans = {}
         for e in entries:
             self._tables.pop(e, None)
@@ -234,8 +250,8 @@ class PromptCache:
         """another pool size (at least the used pages): the used pages move to the front of the new pool.  Waits for the
         device; graphs captured over the old pool must not be replayed."""
         import torch
-        if n_pages < 1:
-            raise ValueError(f"PromptCache.resize: n_pages must be positive, got {n_pages}")
+        if not 1 <= n_pages < 1 << 31:
+            raise ValueError(f"PromptCache.resize: n_pages must be positive (and an int32), got {n_pages}")
         pages = torch.zeros((n_pages, *self.pages.shape[1:]), dtype=self.dtype, device=self.device)
         self._tables = {}
         rc = self._lib.mi_prompt_cache_resize(self._h, pages.data_ptr(), n_pages, self._stream())
@@ -245,6 +261,7 @@ class PromptCache:
 
     # -- what is held -----------------------------------------------------------
     def length(self, entry: int) -> int:
+        _int32("length", entry)
         n = c_int32()
         _check(self._lib.mi_prompt_cache_entry(self._h, entry, ctypes.byref(n), None, 0))
         return n.value
@@ -255,6 +272,7 @@ class PromptCache:
         if known is not None:
             full, last = known
             return full + [last] if last >= 0 else full[:]
+        _int32("table", entry)
         cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
         _check(self._lib.mi_prompt_cache_entry(self._h, entry, ctypes.byref(n), t, cap))
@@ -284,6 +302,8 @@ class PromptCache:
         hold; in a new output they are zeros).  Inference only: no gradient."""
         import torch
         hd, kv, dtype, device = self.head_dim, self.n_kv_heads, self.dtype, self.device
+        if not 0 <= entry < 1 << 31 or not 0 <= layer < 1 << 31:
+            raise RuntimeError(f"mi_prompt_cache: prompt attention: no entry {entry}, layer {layer}")
         if q.dim() != 3 or q.shape[2] != hd:
             raise ValueError(f"PromptCache.attention: q [tokens, heads, {hd}], got {tuple(q.shape)}")
         if (k is None) != (v is None):

@@ -70,3 +70,11 @@ def test_the_argument_block_is_the_headers_struct(pc):
     vals = list(range(1, len(fields) + 1))
     s = S.from_buffer_copy(pc._ATTN.pack(*vals))
     assert [int(getattr(s, f)) for f, _ in fields] == vals
+
+
+@pytest.mark.parametrize("change", [dict(n_layers=2 ** 32 + 1), dict(n_kv_heads=2 ** 32 + 2), dict(n_pages=2 ** 32 + 4), dict(max_entries=2 ** 32 + 1),
+                                    dict(max_tokens=2 ** 32 + 1), dict(max_tokens=-1)])
+def test_configurations_beyond_32_bits(pc, change):
+    """ctypes would cut them to numbers that look right"""
+    with pytest.raises(ValueError, match="int32"):
+        pc.PromptCache(**{**dict(n_layers=2, n_kv_heads=2, head_dim=64, n_pages=4), **change})

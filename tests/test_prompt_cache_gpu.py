@@ -1053,3 +1053,24 @@ def test_the_per_thread_stream_is_another_one_in_every_thread(pc):
     [t.join() for t in ts]
     torch.cuda.synchronize()
     assert steps[1] is True and torch.equal(out, want) and (cache.pages == 0).all()
+
+
+def test_numbers_beyond_32_bits_are_refused(pc):
+    """ctypes would cut them: reserve(e, 2^32 + 5) was five tokens, write(start=2^32) the first one"""
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [3])
+    want, big = cache.attention(e, 1, q, k, v), 1 << 32
+    t = torch.zeros(2, 3, 2, 64, dtype=BF, device="cuda")
+    for f in (lambda: cache.reserve(e, big + 5), lambda: cache.reserve(e + big, 5), lambda: cache.write(e, t, t, big), lambda: cache.write(e, t, t, 0, layer=big),
+              lambda: cache.write(e + big, t, t, 0), lambda: cache.extend(e + big, t, t), lambda: cache.fork(e + big), lambda: cache.copy(e - big),
+              lambda: cache.free(e + big), lambda: cache.free([e, e - big]), lambda: cache.resize(big + 40), lambda: cache.length(e + big), lambda: cache.table(e + big)):
+        with pytest.raises(ValueError, match="int32"):
+            f()
+    with pytest.raises(RuntimeError, match="max_entries"):
+        cache.fork(e, 1 << 40)
+    for entry, layer in ((e + big, 1), (e, 1 + big), (e - big, 1)):
+        with pytest.raises(RuntimeError, match="no entry"):
+            cache.attention(entry, layer, q, k, v)
+    assert cache.length(e) == 70 and torch.equal(cache.attention(e, 1, q, k, v), want)
+    many = k[:1, :, :].as_strided((2 ** 31 - 8, 2, 64), (0, 64, 1))
+    with pytest.raises(RuntimeError, match="2\\^31 keys"):
+        cache.attention(e, 1, q, many, many, dev([0, 3]), dev([0, 3]))
