@@ -76,7 +76,7 @@ def _check(rc: int):
 
 
 def _int32(what, *numbers):
-    """refuses what ctypes would cut to 32 bits"""
+    """refuses what ctypes would cut to 32 bits (n >> 31 is 0 for the ordinary ones: the short way past it)"""
     for n in numbers:
         if not -1 << 31 <= n < 1 << 31:
             raise ValueError(f"PromptCache.{what}: {n} is no int32")
@@ -173,7 +173,8 @@ class PromptCache:
 
     def extend(self, entry: int, k, v) -> None:
         """tokens at the end of the entry: k, v [n_layers, n, n_kv_heads, head_dim].  No gradient."""
-        _int32("extend", entry)
+        if entry >> 31:
+            _int32("extend", entry)
         k, v = self._kv(k, v, "extend")
         if k.shape[0] != self.n_layers:
             raise ValueError(f"PromptCache.extend: keys and values of all {self.n_layers} layers, got {tuple(k.shape)}")
@@ -185,7 +186,9 @@ class PromptCache:
         _check(rc)
 
     def _kv(self, k, v, what):
-        _no_gradient(what, k, v)
+        import torch
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad) or getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0:
+            _no_gradient(what, k, v)
         if k.dim() == 3 and v.dim() == 3:
             k, v = k[None], v[None]
         want = (self.n_kv_heads, self.head_dim)
@@ -206,7 +209,8 @@ class PromptCache:
         a captured `write` reaches) copied"""
         if count < 0:
             raise ValueError(f"PromptCache.fork: count must not be negative, got {count}")
-        _int32("fork", entry)
+        if entry >> 31:
+            _int32("fork", entry)
         if count > self._max_entries:
             raise RuntimeError(f"mi_prompt_cache: prompt cache: more than max_entries ({self._max_entries}) entries")
         out, own, tables = (c_int32 * count)(), (c_int32 * count)(), self._tables
@@ -221,7 +225,8 @@ class PromptCache:
 
     def copy(self, entry: int) -> int:
         """a new entry with the same tokens in pages of its own"""
-        _int32("copy", entry)
+        if entry >> 31:
+            _int32("copy", entry)
         e = c_int32()
         _check(self._lib.mi_prompt_cache_copy(self._h, entry, ctypes.byref(e), self._stream()))
         return e.value
@@ -229,9 +234,10 @@ class PromptCache:
     def free(self, entries) -> None:
         """drops an entry or several; their pages are free once no other entry shares them"""
         entries = [entries] if isinstance(entries, int) else list(entries)
-        _int32("free", *entries)
         self._plans = {}
         for e in entries:
+            if e >> 31:
+                _int32("free", e)
             self._tables.pop(e, None)
         rc = self._lib.mi_prompt_cache_free(self._h, len(entries), (c_int32 * len(entries))(*entries), self._stream())
         self._plans = {}
@@ -272,7 +278,8 @@ class PromptCache:
         if known is not None:
             full, last = known
             return full + [last] if last >= 0 else full[:]
-        _int32("table", entry)
+        if entry >> 31:
+            _int32("table", entry)
         cap, n = self._table_cap, c_int32()
         t = (c_int32 * cap)()
         _check(self._lib.mi_prompt_cache_entry(self._h, entry, ctypes.byref(n), t, cap))
@@ -302,7 +309,7 @@ class PromptCache:
         hold; in a new output they are zeros).  Inference only: no gradient."""
         import torch
         hd, kv, dtype, device = self.head_dim, self.n_kv_heads, self.dtype, self.device
-        if not 0 <= entry < 1 << 31 or not 0 <= layer < 1 << 31:
+        if entry >> 31 or layer >> 31:
             raise RuntimeError(f"mi_prompt_cache: prompt attention: no entry {entry}, layer {layer}")
         if q.dim() != 3 or q.shape[2] != hd:
             raise ValueError(f"PromptCache.attention: q [tokens, heads, {hd}], got {tuple(q.shape)}")
