@@ -262,11 +262,11 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
 }
 
 // How a call is cut up: tiles of 128 rows of a key head, and where these do not fill the chip the keys `splits` ways, so that there
-// is a workgroup for each of the 256 CUs -- two, if each still has eight chunks of 64 keys or more: 50 us with 64 splits of the 1024
-// chunks of four tokens behind 65 500, 66 with 32; but 32 with 32 splits of the 82 chunks of 64 single tokens behind 2048, 26 with 16,
-// because every split's partials are written and read again.  Up to 256 rows a split may be one chunk, beyond it is two at least (ten
-// tokens of 12 heads behind 400: 12.1 us with 8 splits of one, 13.2 with 4 of two; but 30 single tokens of 28 heads behind 400 16.6 with
-// 12 splits, 13.6 with 7); up to four chunks go unsplit, where the join costs as much as they do (behind 150: 11.7 us, in two 13.0).
+// is a workgroup for each of the 256 CUs -- two, if each still has eight chunks of 64 keys or more: the 1024 chunks of four tokens
+// behind 65 500 take a third longer with 32 splits than with 64; but the 82 chunks of 64 single tokens behind 2048 a fifth longer with 32
+// than with 16, because every split's partials are written and read again.  Up to 256 rows a split may be one chunk, beyond it is two at
+// least (ten tokens of 12 heads behind 400: 8 % less with 8 splits of one than with 4 of two; but 30 single tokens of 28 heads behind 400
+// 22 % more with 12 splits than with 7); up to four chunks go unsplit, where the join costs as much as they do (behind 150: 11 % more in two).
 struct Plan {
     int splits, tiles;
     int64_t rows;                        // of all key heads

@@ -72,8 +72,8 @@ struct TF16 {
     }
     __device__ static unsigned scaled(unsigned two, float f) { return pack(up((unsigned short)(two & 0xffffu)) * f, up((unsigned short)(two >> 16)) * f); }
     __device__ static unsigned short down(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
-    // f16 loses what is below 2^-25: the probabilities are held as 2^7 p (p <= 1), so that a long tail of small ones keeps its
-    // weight; the factor cancels in o / sum
+    // f16 loses what is below 2^-25: the probabilities are held as 2^7 p, so that a long tail of small ones keeps its weight; the factor
+    // cancels in o / sum.  p stays below 2^8 (the maximum may lag by that), so what is held below 2^15, half of f16's largest value
     static constexpr float shift = 7.f;
 };
 
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool prompt_own_range(const PromptArgs &a, Ints cu_q,
 // ---------------------------------------------------------------------------------------------------------------------
 // One row by one wave: lanes over the keys of a step for the scores, over the head's dims for the output.  Sees exactly the
 // row's keys, so nothing that is masked is ever read.  64 keys cost ~1 us: for the rows of the kernel
-// below in which a masked value that is no number would have entered a product (0 x inf).
+// below in which a value that is no number has entered a product with a probability rounded to 0 or masked (0 x inf).
 // ---------------------------------------------------------------------------------------------------------------------
 template <class T, int HD>
 __device__ void prompt_row(const PromptArgs &a, int token, int head, int64_t p0, int64_t p1, int64_t lo, int64_t hi, float *qs /* [HD] of this wave */,
@@ -218,7 +218,8 @@ __device__ void prompt_row(const PromptArgs &a, int token, int head, int64_t p0,
 // A masked key has p = 0 exactly (so have the rows behind the prompt's and the texts' end, which hold the last one again), a rounding may
 // leave one of 0 or less, and 0 x (inf or NaN in V) would be NaN: a row whose result is no finite number is done again by prompt_row,
 // which reads only what the row sees and keeps its probabilities in f32 -- unless its sum is NaN: the sum is over keys that the row
-// sees, so every dim is NaN.
+// sees, so every dim is NaN.  Slow where it is all rows: an infinity in V of a prompt of 4096 takes 13.1 k tokens from 1.05 to 294 ms, one
+// in V of 400 32.7 k tokens from 0.2 to 39 (a NaN in the prompt's K costs nothing).
 // ---------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) bf16_t lds_t;
 // 64 lanes x 16 bytes from base + the lane's offset -> 1 KiB at dst (the same in every lane)
@@ -318,22 +319,21 @@ __device__ __forceinline__ void prompt_finish(const f32x16 (&o)[HD / 32], float 
 
 // TWO: the probabilities enter the product with V in two parts (what the type holds of them, and of the rest), which leaves the
 // output's own rounding as the only one in 16 bits; one part costs another half step of the type on every output (error against 64
-// bits 0.0024 instead of 0.0017 in bf16).  Taken where a key head's rows are two tiles at most, which latency and the reading of the
-// pages bound: 8.6 us instead of 8.0 on ten tokens behind 37, 26.4 instead of 24.8 on 64 single tokens of 32 heads behind 2048.  More
-// rows are bound by the products: 66 instead of 53 on 40 tokens of 64 heads behind 20 000, 1347 instead of 1018 on 13.1 k behind 4096.
-// Four waves also where one holds all the rows: the others bring their quarter of the keys in.  Against workgroups of one and of two
-// waves: 8.6 us instead of 10.5 and 10.0 on ten tokens behind 37, 50 instead of 57 and 55 on four tokens behind 65 500; eight waves
-// took 9.0 and 70.
+// bits 0.0023 instead of 0.0017 in bf16, 0.00029 instead of 0.00021 in f16).  Taken where a key head's rows are two tiles at most, which
+// latency and the reading of the pages bound: 7 % longer than one part on ten tokens behind 37, 6 % on 64 single tokens of 32 heads behind
+// 2048.  More rows are bound by the products: 25 % longer on 40 tokens of 64 heads behind 20 000, 32 % on 13.1 k behind 4096.
+// Four waves also where one holds all the rows: the others bring their quarter of the keys in.  Workgroups of one and of two
+// waves take 22 % and 16 % longer on ten tokens behind 37, 14 % and 10 % on four tokens behind 65 500, eight waves 5 % and 40 %.
 // Two stages of LDS, so that two workgroups share a CU and overlap each other: four stages and one workgroup a CU took 1.7 times as
 // long on four tokens behind 65 500 and 2 % longer on 13.1 k behind 4096, and four stages beside two workgroups (head dim 64) 4 %
 // longer on 4 k tokens of 16 heads behind 1000.
 // What bounds it, and what it takes with its join, launches included:
 //   few rows, short prompt    latency: launch, arguments, bounds and Q, first page, two chunks, store; 8.9 us (10 tokens behind 37)
-//   few rows, long prompt     reading the pages: 57 us for the 269 MB of 65 500 tokens (the kernel 47: 5.7 TB/s); 24 us for 64
-//                             single tokens with pasts (35 MB) behind 2048: 18 + 5.7 for the partials of 16 splits
-//   many rows                 matrix and vector work in turn at the clock that the power limit leaves (1.8 GHz): 990 us for 13.1 k
-//                             tokens of 32 heads of 128 behind 4096, 920 TFLOP/s (products alone, without the exponentials, 652 us);
-//                             head dim 64: the exponentials, 40 us for 4 k tokens of 16 heads behind 1000
+//   few rows, long prompt     reading the pages: 58 us for the 269 MB of 65 500 tokens (the kernel 46: 5.8 TB/s); 24 us for 64
+//                             single tokens with pasts (35 MB) behind 2048, of which 5.7 for the partials of 16 splits
+//   many rows                 matrix and vector work in turn: 1050 us for 13.1 k tokens of 32 heads of 128 behind 4096, 870 TFLOP/s, at the
+//                             1.83 GHz of 2.4 that the power limit leaves, the matrix pipes busy 49 % of the cycles (products alone, without
+//                             the exponentials, 652 us); head dim 64: the exponentials, 40 us for 4 k tokens of 16 heads behind 1000
 template <class T, int HD, bool VT, bool TWO>
 __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArgs a) {
     constexpr int NW = PA_WAVES, KC = PC_PAGE, NKK = HD / 16, NDT = HD / 32, SL = HD / 8;      // keys of a chunk, MFMA steps over hd, output tiles, slots of a row
@@ -629,9 +629,9 @@ __global__ void __launch_bounds__(64 * PA_WAVES, 2) prompt_tile_kernel(PromptArg
 
 // the splits' partials of a row -> the output: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  HD / 4 lanes hold four dims each; PAR
 // such groups take every PAR-th split of a row and meet in LDS, always in the same order.  One group up to 8 splits: all of its loads
-// are in flight at once (128 single tokens: 31 us with their tiles, 33 with four groups); four beyond, where one would go through them
-// as a chain (34 us at 64 splits) and eight are too many workgroups (64 single tokens behind 2048: 26.8 instead of 25.5).  Bound by
-// latency (5.2 us for 128 rows x 64 splits of 128 dims) and by the L2s' 17 MB of partials (5.7 us for 2048 rows x 16 splits: 3 TB/s).
+// are in flight at once (128 single tokens take 6 % longer, their tiles included, with four groups); four beyond, where one would go
+// through them as a chain (34 us at 64 splits, four 5.5) and eight are too many workgroups (64 single tokens behind 2048: 5 % longer).
+// Bound by latency (5.5 us for 128 rows x 64 splits of 128 dims) and by the L2s' 17 MB of partials (5.7 us for 2048 rows x 16 splits: 3 TB/s).
 template <class T, int HD, int PAR>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR / PAR;                           // lanes of a group, rows of a workgroup
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(256) pc_table_kernel(PcTableArgs a) {
 }
 
 // keys and values of n tokens into the pages of an entry: a thread per (layer, token, key head, 8 dims) and K / V.  4000 tokens of 28
-// layers (229 MB read and written): 36 us, 6.4 TB/s; 37 tokens: 3.2 us.
+// layers (229 MB read and written): 36 us, 6.3 TB/s; 37 tokens: 3.2 us.
 // k_inter: the source's dims are interleaved by rotary pair (2 f + h = pair f, half h); v_dim != 1: the source is V^T, elements
 // v_dim apart.  Both only where the encoder stores a prompt, once.
 struct PcWriteArgs {
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(256) pc_write_kernel(PcWriteArgs a) {
 // the first `rows` rows of every (layer, key head, K / V) of page src[j] -> page dst[j].  grid (blocks, jobs): a thread takes four
 // words, so that a launch of a few pages fills the chip too.  200 pages of 28 layers (734 MB read and written): 128 us, 5.7 TB/s, with
 // the words of the tables where the pages move (a launch of their own took 4.6 us for 200 moves in 1600 words, latency); 200
-// copies of 40 rows of one page: 35 us; four: 4.0.
+// copies of 40 rows of one page: 35 us; four: 4.1.
 struct PcCopyArgs {
     const bf16_t *from;
     bf16_t *to;

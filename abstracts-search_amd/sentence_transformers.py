@@ -486,16 +486,17 @@ class SentenceTransformer:
     # Embeddings do not depend on which sequences share a pass beyond bf16 / f32 rounding order (tests: batching
     # invariance).  `token_budget = None`: passes of exactly `batch_size` length-sorted sequences.
     token_budget = 32768
-    # Texts behind a cached prompt that make one pass of the same cost with the prompt's tokens as without go without the cache: up to
+    # Texts behind a cached prompt whose passes cost the same with the prompt's tokens go without the cache: passes of up to
     # 48 tokens in all (the query-time path streams every weight once either way, and may have the attention inside its O
-    # projection: a query of 31 tokens 1.09 ms, of its own 11 behind 20 cached ones 1.21), or more than 64 of their own and up to 384
-    # in all (passes of 70 to 400 tokens cost 2.7 - 3.3 ms, by how their rows fall on the tiles: 8 texts of 15 tokens behind 24 2.71
-    # against 3.19 cached, one of 100 behind 200 3.18 against 3.39; but of 60 behind 200 3.10 against 2.40, four of 40 behind 60 3.14
-    # against 2.83, 16 of 15 behind 32 3.50 against 3.20).
+    # projection: a query of 31 tokens 1.07 ms, of its own 11 behind 20 cached ones 1.19), or of more than 64 of their own and up to 384
+    # in all (passes of 70 to 400 tokens cost 2.7 - 3.3 ms, by how their rows fall on the tiles: 8 texts of 15 tokens behind 24 2.69
+    # against 3.18 cached, one of 100 behind 200 3.17 against 3.39; but of 60 behind 200 3.09 against 2.38, four of 40 behind 60 3.04
+    # against 2.83, 16 of 15 behind 32 3.36 against 3.20).  Measured on stella's shape, on which it is not always the better side
+    # either: 16 of 15 behind 20 take 2.97 without the cache, 3.20 with it.
     prompt_break_even = (48, 64, 384)
     # Texts behind different cached prompts cannot share a pass, without the cache they can: what a pass costs besides its tokens, in
-    # tokens (half of it all told on the query-time path).  Passes of 70 / 300 / 1000 / 10 000 tokens take 2.8 / 2.9 / 5.0 / 24.7 ms, one
-    # of up to 48 1.1: 2.4 us a token and 2.4 ms, the weights' streaming, which grows with the model as the tokens' share does.
+    # tokens (half of it all told on the query-time path).  Passes of 70 / 300 / 1000 / 10 000 tokens take 2.8 / 2.9 / 4.8 / 24.2 ms, one
+    # of up to 48 1.1 - 1.2: 2.3 us a token and 2.4 ms, the weights' streaming, which grows with the model as the tokens' share does.
     prompt_pass_tokens = 1000
 
     def _groups(self, token_lists, cached, batch_size):
@@ -525,8 +526,8 @@ class SentenceTransformer:
             else:
                 prompted.append((rest - total, rest, handle, members))
         # many prompts with little behind each: the ones that save the fewest tokens go together, with their tokens, where that is
-        # cheaper by an eighth at least (two prompts of 160 tokens with one text of 5 each 2.5 ms cached, 3.0 together; four 5.1 and 3.7,
-        # thirty 38 and 15; thirty with eight texts of 60 each 103 and 123)
+        # cheaper by an eighth at least (two prompts of 160 tokens with one text of 5 each 2.5 ms cached, 3.0 together; four 5.0 and 3.5,
+        # thirty 38 and 14; thirty with eight texts of 60 each 100 and 120)
         if len(prompted) > 1:
             prompted.sort(key=lambda g: g[0])                                   # (the greatest savings first)
             keep, best = len(prompted), None

@@ -196,7 +196,8 @@ int mi_prompt_cache_used(mi_prompt_cache *c, int32_t *used_pages, int32_t *entri
  * than queries the first ones are the text's past: one query per text is the single-token form).  causal: query number a of
  * a text sees its keys 0 .. a + keys - queries; otherwise all of them.  A query that sees nothing (empty prompt, no key)
  * gets zeros.  n_heads is a multiple of the cache's n_kv_heads: head h reads key head h / (n_heads / n_kv_heads).
- * Masked keys and values may hold anything, infinities and NaN too. */
+ * Masked keys and values may hold anything, infinities and NaN too.  Sums are f32; where a key head's rows (tokens x heads of its group)
+ * are more than 256, a probability is rounded to the tensors' type before its product with V, up to there it is kept in two parts. */
 typedef struct mi_prompt_attn {
     int32_t entry, layer;
     int32_t n_heads;
@@ -205,7 +206,7 @@ typedef struct mi_prompt_attn {
     const void *k, *v;               /* [n_keys][n_kv_heads][head_dim]; may be NULL with n_keys = 0 */
     void *out;                       /* [n_tokens][n_heads][head_dim] */
     int64_t q_token, q_head;         /* strides in elements, multiples of 8; head_dim is contiguous */
-    int64_t k_token, k_head, v_token, v_head, o_token, o_head;
+    int64_t k_token, k_head, v_token, v_head, o_token, o_head;   /* k_token, v_token: 0 .. 2^23 - 1 */
     const int32_t *cu_q, *cu_k;      /* device, [n_texts + 1], not decreasing; both NULL: one text */
     int32_t causal;
     float scale;                     /* 1 / sqrt(head_dim) as a rule */

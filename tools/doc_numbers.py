@@ -1,5 +1,5 @@
 """Regenerate the number tables that head DESIGN.md and README.md from ONE bench line (the closing commit's `python bench.py`):
-   python tools/doc_numbers.py profiles/r06_cfg4_bench_final.json
+   python tools/doc_numbers.py profiles/cfg4_bench_line.json
 Idempotent: the rows between the table header and the first non-table line are replaced.  No hand-copied figures."""
 import json, os, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
