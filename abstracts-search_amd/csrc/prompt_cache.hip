@@ -246,6 +246,7 @@ PromptArgs attention_args(mi_prompt_cache *c, const mi_prompt_attn &x, const Pro
     for (const void *p : {x.q, x.k, x.v, static_cast<const void *>(x.out)}) MI_REQUIRE(aligned16(p), "prompt attention: tensors must be 16-byte aligned");
     for (int64_t s : {x.q_token, x.q_head, x.k_token, x.k_head, x.v_token, x.v_head, x.o_token, x.o_head})
         MI_REQUIRE(s % 8 == 0, "prompt attention: strides must be multiples of 8 elements");
+    MI_REQUIRE((x.n_tokens <= 1 || x.o_token) && (x.n_heads == 1 || x.o_head), "prompt attention: rows of out are the same memory");
     MI_REQUIRE(std::max(std::abs(x.k_token), std::abs(x.v_token)) < 1 << 23 && x.k_token >= 0 && x.v_token >= 0,
                "prompt attention: tokens of k and v must be less than 2^23 elements apart");
     PromptArgs a{};

@@ -138,7 +138,7 @@ int mi_enc_gemm_bf16(int device, int M, int N, int K, const void *A, const void 
  * them behind its writes (as with any device buffer); pages of entries that other streams read, or that a captured graph
  * reads, are given out again only after the device has been waited for.  mi_prompt_attention and mi_prompt_cache_write may be
  * captured into a graph (a replay uses the entry's length as it was at the capture; the entry must live, page moves by
- * mi_prompt_cache_compact are followed, a resize ends its use); the other calls are refused on a stream that is being captured.
+ * mi_prompt_cache_compact are followed -- by replays that the caller orders behind them --, a resize ends its use); the other calls are refused on a stream that is being captured.
  * A stream that entries were made or freed on must have finished its work when it is destroyed; on the per-thread handle, which is another
  * stream in every thread, whatever is handed on is waited for.
  * A capture that another thread has open is left alone: no call here fails because of it or ends it, also where it waits.
@@ -206,7 +206,7 @@ typedef struct mi_prompt_attn {
     const void *k, *v;               /* [n_keys][n_kv_heads][head_dim]; may be NULL with n_keys = 0 */
     void *out;                       /* [n_tokens][n_heads][head_dim] */
     int64_t q_token, q_head;         /* strides in elements, multiples of 8; head_dim is contiguous */
-    int64_t k_token, k_head, v_token, v_head, o_token, o_head;   /* k_token, v_token: 0 .. 2^23 - 1 */
+    int64_t k_token, k_head, v_token, v_head, o_token, o_head;   /* k_token, v_token: 0 .. 2^23 - 1; o_token, o_head: not 0 */
     const int32_t *cu_q, *cu_k;      /* device, [n_texts + 1], not decreasing; both NULL: one text */
     int32_t causal;
     float scale;                     /* 1 / sqrt(head_dim) as a rule */

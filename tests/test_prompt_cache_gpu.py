@@ -1074,3 +1074,48 @@ def test_numbers_beyond_32_bits_are_refused(pc):
     many = k[:1, :, :].as_strided((2 ** 31 - 8, 2, 64), (0, 64, 1))
     with pytest.raises(RuntimeError, match="2\\^31 keys"):
         cache.attention(e, 1, q, many, many, dev([0, 3]), dev([0, 3]))
+
+
+def test_a_captured_write_waits_for_the_readers_of_a_page_that_was_shared(pc):
+    """with the reading still under way when the write is captured (torch's own capture would have waited for it)"""
+    import ctypes
+    hip, V = ctypes.CDLL("libamdhip64.so"), ctypes.c_void_p
+    cache = pc.PromptCache(1, 1, 64, 4, max_entries=6)
+    kv, q = torch.randn(1, 64, 1, 64, device="cuda", dtype=BF), torch.randn(1, 2, 64, device="cuda", dtype=BF)
+    nothing, out, side, s = kv * 0, torch.empty_like(q), torch.cuda.Stream(), torch.cuda.Stream()
+    parent = cache.new()
+    cache.extend(parent, kv, kv)
+    want = cache.attention(parent, 0, q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        kid = cache.fork(parent)[0]
+        torch.cuda._sleep(20_000_000)
+        cache.attention(kid, 0, q, out=out)
+        cache.free(kid)
+        read = torch.cuda.Event()
+        read.record()
+    graph, exe = V(), V()
+    assert hip.hipStreamBeginCapture(V(s.cuda_stream), 2) == 0
+    with torch.cuda.stream(s):
+        cache.write(parent, nothing, nothing, 0)
+        done = read.query()
+    assert hip.hipStreamEndCapture(V(s.cuda_stream), ctypes.byref(graph)) == 0 and done
+    assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, ctypes.c_size_t(0)) == 0
+    for _ in range(3):
+        assert hip.hipGraphLaunch(exe, V(s.cuda_stream)) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and (cache.pages[0] == 0).all()
+        cache.pages[0] = 1
+    assert hip.hipGraphExecDestroy(exe) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+def test_the_library_refuses_an_output_whose_rows_are_the_same_memory(pc):
+    cache, e, pk, pv, q, k, v, cu_q, cu_k = make(pc, BF, 4, 2, 64, 70, [3])
+    out = torch.zeros_like(q)
+    for o_token, o_head, ok in ((256, 64, True), (0, 64, False), (256, 0, False)):
+        a = pc._ATTN.pack(e, 1, 4, 3, 3, 1, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 256, 64, 128, 64, 128, 64, o_token, o_head, 0, 0, 1, 0.125, 0, 0, 0, 0)
+        rc = pc._Lib.get().mi_prompt_attention(cache._h, a, None)
+        assert (rc == 0) == ok and (ok or b"same memory" in pc._Lib.get().mi_enc_last_error())
+    o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
+    torch.cuda.synchronize()
+    close(out, o, b)
