@@ -1119,3 +1119,89 @@ def test_the_library_refuses_an_output_whose_rows_are_the_same_memory(pc):
     o, b = reference_many(q, pk, pv, k, v, cu_q, cu_k, True)
     torch.cuda.synchronize()
     close(out, o, b)
+
+
+def test_several_threads_on_one_cache(pc):
+    """four threads store, fork, read, copy, write and free prompts on streams of their own while a fifth moves pages: every output is
+    what its prompt gives"""
+    import threading
+    cache = pc.PromptCache(2, 2, 64, 120, max_entries=100, max_tokens=64 * 20)
+    rng = np.random.default_rng(5)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kv = [[torch.randn(2, n, 2, 64, generator=g, device="cuda").to(BF) for _ in range(2)] for n in (1, 63, 64, 130, 200, 320, 700)]
+    q = torch.randn(5, 4, 64, generator=g, device="cuda").to(BF)
+    own = [torch.randn(5, 2, 64, generator=g, device="cuda").to(BF) for _ in range(2)]
+    want = []
+    for k, v in kv:
+        e = cache.new()
+        cache.extend(e, k, v)
+        want.append(cache.attention(e, 1, q, *own))
+        cache.free(e)
+    torch.cuda.synchronize()
+    outs, errors, stop = [], [], threading.Event()
+
+    def run(seed):
+        r = np.random.default_rng(seed)
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                held = []
+                for _ in range(150):
+                    op = r.integers(0, 6)
+                    try:
+                        if op < 2 or not held:
+                            i, e = int(r.integers(0, len(kv))), cache.new()
+                            held.append((e, i))
+                            k, v = kv[i]
+                            half = k.shape[1] // 2
+                            cache.extend(e, k[:, :half], v[:, :half])
+                            cache.extend(e, k[:, half:], v[:, half:])
+                        else:
+                            e, i = held[int(r.integers(0, len(held)))]
+                            if op == 2:
+                                held += [(c, i) for c in cache.fork(e, int(r.integers(1, 4)))]
+                            elif op == 3:
+                                held.append((cache.copy(e), i))
+                            elif op == 4:
+                                k, v = kv[i]
+                                last = (k.shape[1] - 1) // 64 * 64
+                                if k.shape[1] % 64:                   # (the same tokens once more, in the page that is the entry's own)
+                                    cache.write(e, k[:, last:], v[:, last:], last)
+                            else:
+                                held.remove((e, i))
+                                cache.free(e)
+                    except RuntimeError as err:                   # a full pool: half of what is held goes
+                        assert "free" in str(err) or "max_entries" in str(err), err
+                        bad = [h for h in held if cache.length(h[0]) != kv[h[1]][0].shape[1]]
+                        gone = bad + [h for h in held if h not in bad][::2]
+                        cache.free([e for e, _ in gone])
+                        held = [h for h in held if h not in gone]
+                        continue
+                    for e, i in held[-2:]:
+                        outs.append((i, cache.attention(e, 1, q, *own)))
+                cache.free([e for e, _ in held])
+        except Exception as err:                                  # pragma: no cover
+            errors.append(err)
+
+    def move():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not stop.is_set():
+                    cache.compact()
+                    if rng.random() < 0.2:
+                        try:
+                            cache.resize(int(rng.integers(120, 140)))
+                        except RuntimeError as err:               # (fewer than are used)
+                            assert "in use" in str(err), err
+        except Exception as err:                                  # pragma: no cover
+            errors.append(err)
+
+    ts = [threading.Thread(target=run, args=(s,)) for s in range(4)]
+    mover = threading.Thread(target=move)
+    [t.start() for t in ts + [mover]]
+    [t.join() for t in ts]
+    stop.set()
+    mover.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert len(outs) > 500 and all(torch.equal(o, want[i]) for i, o in outs)
+    assert cache.used_pages == 0
