@@ -377,10 +377,10 @@ int mi_prompt_cache_create(const mi_prompt_cache_cfg *cfg, int device, void *pag
         BesideCaptures beside;
         if (!pages) {                    // zeros: what a reserved token holds before it is written is at least finite
             pages = c->own.reserve(bytes);
-            zero(pages, bytes, nullptr);
+            zero(pages, bytes, hipStreamPerThread);
         }
         c->pages = static_cast<bf16_t *>(pages);
-        zero(c->tables.reserve(tbytes), tbytes, nullptr);          // (every word of a table is a page number, whatever is read)
+        zero(c->tables.reserve(tbytes), tbytes, hipStreamPerThread);   // (every word of a table is a page number, whatever is read)
         wait_for_device();
         c->ref.assign(g.n_pages, 0);
         c->tag.assign(g.n_pages, ANY);

@@ -356,7 +356,6 @@ class SentenceTransformer:
 
     def load_weights(self, weights: dict):
         """name -> torch tensor / numpy array (f32, bf16 or f16; host or CUDA)."""
-        import torch
         with self._prompts_lock:                 # (a prompt that another thread caches waits for the new weights)
             self._drop_prompts()
             return self._load_weights(weights)
@@ -446,8 +445,9 @@ class SentenceTransformer:
         `prompts` (None: the default prompt).  Causal models only -- in a bidirectional one (stella, gte-Qwen2) the prompt's
         hidden states depend on the text behind it.  Returns how many tokens are held; the embeddings are the same to bf16
         rounding.  A text whose tokens do not begin with a cached prompt is encoded as before, and so are few texts behind a
-        short prompt (`prompt_break_even`) and single texts behind many prompts (`prompt_pass_tokens`), where that is faster.  A prompt that begins as one that is cached shares its pages.
-        `load_weights` drops all of them."""
+        short prompt (`prompt_break_even`) and single texts behind many prompts (`prompt_pass_tokens`), where that is faster.  A
+        prompt that begins as one that is cached shares its pages.  `load_weights` drops all of them.  Other threads may encode
+        meanwhile."""
         import torch
         if not self.config.get("causal"):
             raise ValueError("cache_prompt needs a causal model: in a bidirectional one the prompt's hidden states depend on the text behind it")
@@ -597,9 +597,9 @@ class SentenceTransformer:
         # straight to row sel[i] of `out`): the packing of the next pass overlaps the GPU running this one
         for sel in self._passes(sorted(members, key=lambda i: -len(token_lists[i])), token_lists, batch_size):
             cu = np.zeros(len(sel) + 1, np.int32)
-            cu[1:] = np.cumsum([len(token_lists[i]) for i in sel])
-            if isinstance(token_lists[sel[0]], np.ndarray):
-                ids = np.concatenate([np.ascontiguousarray(token_lists[i], np.int32) for i in sel])
+            np.cumsum([len(token_lists[i]) for i in sel], out=cu[1:])
+            if isinstance(token_lists[sel[0]], np.ndarray):           # id arrays (what `tokenizers` can hand over)
+                ids = np.concatenate([token_lists[i] for i in sel]).astype(np.int32, copy=False)
             else:
                 ids = np.fromiter(itertools.chain.from_iterable(token_lists[i] for i in sel), np.int32, count=int(cu[-1]))
             rows = np.asarray(sel, np.int32)

@@ -138,10 +138,11 @@ int mi_enc_gemm_bf16(int device, int M, int N, int K, const void *A, const void 
  * them behind its writes (as with any device buffer); pages of entries that other streams read, or that a captured graph
  * reads, are given out again only after the device has been waited for.  mi_prompt_attention and mi_prompt_cache_write may be
  * captured into a graph (a replay uses the entry's length as it was at the capture; the entry must live, page moves by
- * mi_prompt_cache_compact are followed -- by replays that the caller orders behind them --, a resize ends its use); the other calls are refused on a stream that is being captured.
- * A stream that entries were made or freed on must have finished its work when it is destroyed; on the per-thread handle, which is another
- * stream in every thread, whatever is handed on is waited for.
- * A capture that another thread has open is left alone: no call here fails because of it or ends it, also where it waits.
+ * mi_prompt_cache_compact are followed by replays that the caller orders behind them, a resize ends its use); the other calls
+ * are refused on a stream that is being captured.  A stream that entries were made or freed on must have finished its work when
+ * it is destroyed; on the per-thread handle, which is another stream in every thread, whatever is handed on is waited for.
+ * A capture that another thread has open is left alone: no call here fails because of it or ends it, also where it waits (work on
+ * the null stream excepted while a blocking stream is captured: HIP refuses it).
  * ------------------------------------------------------------------------------------------------------------------- */
 #define MI_PROMPT_PAGE 64
 

@@ -710,17 +710,24 @@ def test_refusals(pc):
 class OpenCapture:
     """another thread captures a stream in global mode while the body runs; `ended`: what hipStreamEndCapture returned"""
 
+    def __init__(self, blocking=False):
+        self.blocking = blocking
+
     def __enter__(self):
         import ctypes
         import threading
         hip, V = ctypes.CDLL("libamdhip64.so"), ctypes.c_void_p
-        self.leave, opened, side = threading.Event(), threading.Event(), torch.cuda.Stream()
+        self.leave, opened, side = threading.Event(), threading.Event(), torch.cuda.Stream().cuda_stream
+        if self.blocking:
+            made = V()
+            assert hip.hipStreamCreate(ctypes.byref(made)) == 0
+            side = made.value
 
         def run():
-            self.began = hip.hipStreamBeginCapture(V(side.cuda_stream), 0)
+            self.began = hip.hipStreamBeginCapture(V(side), 0)
             opened.set()
             self.leave.wait(60)
-            self.ended = hip.hipStreamEndCapture(V(side.cuda_stream), ctypes.byref(V()))
+            self.ended = hip.hipStreamEndCapture(V(side), ctypes.byref(V()))
             hip.hipGetLastError()
 
         self.thread = threading.Thread(target=run, daemon=True)
@@ -769,6 +776,11 @@ def test_captures_of_other_threads_are_left_alone(pc):
         pc._check(pc._Lib.get().mi_prompt_cache_destroy(raw))
     assert c.ended == 0
     torch.cuda.synchronize()
+    with OpenCapture(blocking=True) as c:                                          # (beside which the null stream may not be used)
+        pc._check(pc._Lib.get().mi_prompt_cache_create(pc.ctypes.byref(pc._Cfg(1, 1, 64, 1, 4, 2, 0)), 0, None, pc.ctypes.byref(raw)))
+        pc._check(pc._Lib.get().mi_prompt_cache_resize(raw, None, 9, side.cuda_stream))
+        pc._check(pc._Lib.get().mi_prompt_cache_destroy(raw))
+    assert c.ended == 0
     assert all(torch.equal(x, want) for x in got)
     assert (cache.pages[cache.table(e)[0]] == 0).all()
 
